@@ -7,5 +7,5 @@ from . import _cabi  # noqa: F401
 
 __all__ = [
     "rmsnorm", "gqa_decode", "mla_decode", "mla_prefill", "dsa_indexer", "dsa_attention", "moe",
-    "gdn_decode", "gdn_prefill", "gemm",
+    "gdn_decode", "gdn_prefill", "gemm", "rope", "qk_norm_rope", "paged_decode", "kv_pages",
 ]

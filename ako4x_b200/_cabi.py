@@ -128,7 +128,34 @@ _SIGNATURES = {
     "ako4x_dsa_indexer_attention_workspace_bytes": (_SZ, [_I64, _I64]),
     "ako4x_dsa_indexer_attention": (_INT, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _F32, _P, _P, _P, _I64, _I64, _I64,
                                             _P, _SZ, _P]),
+    "ako4x_rope": (_INT, [_P, _P, _P, _INT, _P, _I64, _INT, _F32, _P, _P, _I64, _I64, _INT, _P]),
+    "ako4x_qk_norm_rope": (_INT, [_P, _P, _P, _P, _INT, _F32, _P, _INT, _P, _I64, _INT, _F32, _P, _P, _I64, _I64, _INT, _P]),
+    "ako4x_qk_norm_rope_cache": (_INT, [_P, _P, _P, _P, _P, _INT, _F32, _P, _INT, _P, _I64, _INT, _F32, _P, _P, _INT, _P, _P,
+                                        _INT, _I64, _I64, _I64, _I64, _INT, _P]),
+    "ako4x_paged_decode_workspace_bytes": (_SZ, [_I64] * 7),
+    "ako4x_paged_decode": (_INT, [_P, _P, _P, _P, _P, _F32, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _INT, _INT,
+                                  _P, _SZ, _P]),
+    "ako4x_kv_pages_extend_workspace_bytes": (_SZ, [_I64] * 3),
+    "ako4x_kv_pages_extend": (_INT, [_P] * 6 + [_I64] * 5 + [_P, _SZ, _P]),
+    "ako4x_kv_pages_free": (_INT, [_P] * 4 + [_I64] * 5 + [_P]),
+    "ako4x_kv_pages_fork_workspace_bytes": (_SZ, [_I64] * 3),
+    "ako4x_kv_pages_fork": (_INT, [_P] * 3 + [_I64] + [_P] * 6 + [_I64] * 5 + [_P, _SZ, _P]),
+    "ako4x_kv_pages_copy_workspace_bytes": (_SZ, [_I64] * 2),
+    "ako4x_kv_pages_copy": (_INT, [_P] * 3 + [_I64] + [_P] * 3 + [_I64] * 2 + [_P, _SZ, _P]),
+    "ako4x_kv_pages_compact_workspace_bytes": (_SZ, [_I64]),
+    "ako4x_kv_pages_compact": (_INT, [_P] * 3 + [_I64] + [_P] * 3 + [_I64] * 3 + [_P, _SZ, _P]),
 }
+
+
+class HeadRows(ctypes.Structure):
+    """``ako4x_head_rows``: heads of every token, strides in elements."""
+    _fields_ = [("data", _P), ("token_stride", _I64), ("head_stride", _I64), ("heads", _I64)]
+
+
+class KvCache(ctypes.Structure):
+    """``ako4x_kv_cache``: keys or values of a paged cache, strides in elements."""
+    _fields_ = [("data", _P), ("scale", _P), ("page_stride", _I64), ("slot_stride", _I64), ("head_stride", _I64),
+                ("scale_page_stride", _I64), ("scale_slot_stride", _I64), ("scale_head_stride", _I64)]
 
 
 def _declare(l: ctypes.CDLL) -> None:

@@ -18,12 +18,14 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/GradMode.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
 #include <string>
+#include <vector>
 
 #include "ako4x_b200.h"
 
@@ -551,13 +553,449 @@ PyObject* gemm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- New tokens into and through a paged cache -------------------------------------------------
+
+// All tensors of a call on one CUDA device, which is made the current one until the end of the call.
+struct OneDevice {
+  c10::cuda::OptionalCUDAGuard guard;
+  OneDevice(const char* op, std::initializer_list<const Tensor*> all) {
+    const Tensor* first = nullptr;
+    for (const Tensor* t : all) {
+      if (!t || !t->defined()) continue;
+      need(t->is_cuda(), "ako4x_b200 operators take CUDA tensors only (there is no CPU path)");
+      if (!first) first = t;
+      if (t->device() != first->device()) fail(std::string(op) + ": tensors on different devices");
+    }
+    if (first) guard.set_index(first->device().index());
+  }
+};
+Tensor optional(PyObject* o) { return o == Py_None ? Tensor() : tensor(o); }
+int element(ScalarType t) { return t == at::kBFloat16 ? AKO4X_BF16 : t == at::kHalf ? AKO4X_FP16 : AKO4X_E4M3; }
+bool is_index(const Tensor& t) { return t.scalar_type() == at::kInt || t.scalar_type() == at::kLong; }
+
+// [tokens, heads, dim] as it lies where the kernels can read it (heads contiguous, everything at 16 bytes), a
+// contiguous copy otherwise.
+struct HeadRows {
+  Tensor t;
+  ako4x_head_rows r = {};
+  HeadRows() = default;
+  explicit HeadRows(const Tensor& x) : t(x) {
+    auto bad = [&](int d) { return t.size(d) > 1 && (t.stride(d) * 2) % 16 != 0; };
+    if (t.numel() > 0 && ((t.size(2) > 1 && t.stride(2) != 1) || bad(0) || bad(1) || ((uintptr_t)t.data_ptr() & 15))) t = at::empty_like(x, at::MemoryFormat::Contiguous).copy_(x);
+    r.data = t.data_ptr();
+    r.token_stride = t.size(0) > 1 ? t.stride(0) : 0;
+    r.head_stride = t.size(1) > 1 ? t.stride(1) : 0;
+    r.heads = t.size(1);
+  }
+};
+
+struct Rotation {
+  Tensor positions, freq;
+  bool interleaved;
+  float factor;
+  int64_t rotary;
+  Rotation(const char* op, PyObject* pos, PyObject* f, PyObject* inter, PyObject* fac, int64_t tokens, int64_t dim) {
+    positions = tensor(pos);
+    freq = tensor(f);
+    const int truth = PyObject_IsTrue(inter);
+    if (truth < 0) throw python_error();
+    interleaved = truth == 1;
+    factor = (float)number(fac);
+    rotary = 2 * freq.numel();
+    if (!(is_index(positions) && positions.dim() == 1 && positions.size(0) == tokens))
+      fail(std::string(op) + ": positions must be int32 or int64 [tokens]");
+    if (!(freq.scalar_type() == at::kFloat && freq.dim() == 1 && rotary <= dim))
+      fail(std::string(op) + ": inv_freq must be fp32 [rotary_dim / 2] with rotary_dim <= dim");
+    positions = dense(positions);
+    freq = dense(freq);
+  }
+  int wide() const { return positions.scalar_type() == at::kLong; }
+};
+
+void check_rows(const char* op, const Tensor& q, const Tensor& k, const char* names) {
+  const ScalarType dt = q.scalar_type();
+  if (!(q.dim() == 3 && k.dim() == 3 && k.size(0) == q.size(0) && k.size(2) == q.size(2)))
+    fail(std::string(op) + ": " + names + " must be [tokens, heads, dim] with the same tokens and dim");
+  if (!((dt == at::kBFloat16 || dt == at::kHalf) && k.scalar_type() == dt))
+    fail(std::string(op) + ": " + names + " must be bf16 or fp16, of one type");
+  if (!(q.size(2) >= 8 && q.size(2) <= 256 && q.size(2) % 8 == 0))
+    fail(std::string(op) + ": dim must be a multiple of 8 from 8 to 256");
+}
+// Both weights [dim], of the rows' type or fp32 both.
+bool check_weights(const char* op, Tensor& qw, Tensor& kw, const Tensor& q) {
+  bool fp32 = false, any = false;
+  for (Tensor* w : {&qw, &kw}) {
+    if (!w->defined()) continue;
+    if (!(w->dim() == 1 && w->size(0) == q.size(2) && (w->scalar_type() == q.scalar_type() || w->scalar_type() == at::kFloat)))
+      fail(std::string(op) + ": weights must be [dim], of the rows' type or fp32");
+    if (any && fp32 != (w->scalar_type() == at::kFloat)) fail(std::string(op) + ": weights must be of one type");
+    fp32 = w->scalar_type() == at::kFloat;
+    any = true;
+    *w = dense(*w);
+  }
+  return fp32;
+}
+
+// (q, k or None, positions, inv_freq, interleaved, attention_factor)
+PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 6, "rope");
+  c10::NoGradGuard ng;
+  const Tensor &q0 = tensor(a[0]), k0 = optional(a[1]);
+  check_rows("rope", q0, k0.defined() ? k0 : q0, "q and k");
+  const int64_t tokens = q0.size(0), dim = q0.size(2);
+  Rotation rot("rope", a[2], a[3], a[4], a[5], tokens, dim);
+  OneDevice dev("rope", {&q0, &k0, &rot.positions, &rot.freq});
+  HeadRows q(q0), k;
+  Tensor qo = empty(q0.sizes(), q0.scalar_type(), q0), ko;
+  if (k0.defined()) {
+    k = HeadRows(k0);
+    ko = empty(k0.sizes(), k0.scalar_type(), k0);
+  }
+  void *pp = rot.positions.data_ptr(), *fp = rot.freq.data_ptr(), *qp = qo.data_ptr(), *kp = ko.defined() ? ko.data_ptr() : nullptr,
+       *st = current_stream();
+  const int dt = element(q0.scalar_type());
+  check_status(without_gil([&] {
+                 return ako4x_rope(&q.r, ko.defined() ? &k.r : nullptr, pp, rot.wide(), (const float*)fp, rot.rotary, rot.interleaved,
+                                   rot.factor, qp, kp, tokens, dim, dt, st);
+               }),
+               "ako4x_rope");
+  if (ko.defined()) return pack_tuple(std::move(qo), std::move(ko));
+  PyObject* first = pack(std::move(qo));
+  if (!first) throw python_error();
+  PyObject* out = PyTuple_Pack(2, first, Py_None);
+  Py_DECREF(first);
+  return out;
+  END_HANDLE_TH_ERRORS
+}
+
+// (q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved, attention_factor)
+PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 9, "qk_norm_rope");
+  c10::NoGradGuard ng;
+  const Tensor &q0 = tensor(a[0]), &k0 = tensor(a[1]);
+  Tensor qw = tensor(a[2]), kw = tensor(a[3]);
+  check_rows("qk_norm_rope", q0, k0, "q and k");
+  const bool fp32 = check_weights("qk_norm_rope", qw, kw, q0);
+  const int64_t tokens = q0.size(0), dim = q0.size(2);
+  const float eps = (float)number(a[6]);
+  Rotation rot("qk_norm_rope", a[4], a[5], a[7], a[8], tokens, dim);
+  OneDevice dev("qk_norm_rope", {&q0, &k0, &qw, &kw, &rot.positions, &rot.freq});
+  HeadRows q(q0), k(k0);
+  Tensor qo = empty(q0.sizes(), q0.scalar_type(), q0), ko = empty(k0.sizes(), k0.scalar_type(), k0);
+  void *pp = rot.positions.data_ptr(), *fp = rot.freq.data_ptr(), *qp = qo.data_ptr(), *kp = ko.data_ptr(), *qwp = qw.data_ptr(),
+       *kwp = kw.data_ptr(), *st = current_stream();
+  const int dt = element(q0.scalar_type());
+  check_status(without_gil([&] {
+                 return ako4x_qk_norm_rope(&q.r, &k.r, qwp, kwp, fp32, eps, pp, rot.wide(), (const float*)fp, rot.rotary,
+                                           rot.interleaved, rot.factor, qp, kp, tokens, dim, dt, st);
+               }),
+               "ako4x_qk_norm_rope");
+  return pack_tuple(std::move(qo), std::move(ko));
+  END_HANDLE_TH_ERRORS
+}
+
+// A paged cache [pages, page_size, heads, dim] and, in 8 bits, its scales [pages, page_size, heads].
+struct CacheArg {
+  ako4x_kv_cache c = {};
+  CacheArg(const char* op, const Tensor& t, const Tensor& scale, ScalarType rows) {
+    if (t.dim() != 4) fail(std::string(op) + ": caches must be [pages, page_size, heads, dim]");
+    const bool fp8 = t.scalar_type() == at::kFloat8_e4m3fn;
+    if (!fp8 && t.scalar_type() != rows) fail(std::string(op) + ": caches must be of the rows' type or e4m3");
+    if (fp8 != scale.defined()) fail(std::string(op) + ": e4m3 caches, and only those, come with scales");
+    if (fp8 && !(scale.scalar_type() == at::kFloat && shape_is(scale, {t.size(0), t.size(1), t.size(2)})))
+      fail(std::string(op) + ": scales must be fp32 [pages, page_size, heads]");
+    const int64_t to = fp8 ? 16 : 8;   // elements in 16 bytes
+    int64_t st[3];
+    bool fits = t.size(3) <= 1 || t.stride(3) == 1;
+    for (int d = 0; d < 3; ++d) {
+      st[d] = t.size(d) > 1 ? t.stride(d) : 0;
+      fits = fits && st[d] % to == 0;
+    }
+    if (t.numel() > 0 && (!fits || ((uintptr_t)t.data_ptr() & 15)))
+      fail(std::string(op) + ": caches need a contiguous last dimension and strides of whole 16 bytes");
+    c.data = t.data_ptr();
+    c.page_stride = st[0];
+    c.slot_stride = st[1];
+    c.head_stride = st[2];
+    if (fp8) {
+      c.scale = (float*)scale.data_ptr();
+      c.scale_page_stride = scale.size(0) > 1 ? scale.stride(0) : 0;
+      c.scale_slot_stride = scale.size(1) > 1 ? scale.stride(1) : 0;
+      c.scale_head_stride = scale.size(2) > 1 ? scale.stride(2) : 0;
+    }
+  }
+};
+
+// (q, k, v, q_weight, k_weight, positions, inv_freq, slot_mapping, k_cache, v_cache, k_scale, v_scale, eps,
+//  interleaved, attention_factor)
+PyObject* qk_norm_rope_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const char* op = "qk_norm_rope";
+  count(n, 15, op);
+  c10::NoGradGuard ng;
+  const Tensor &q0 = tensor(a[0]), &k0 = tensor(a[1]), &v0 = tensor(a[2]), &slots0 = tensor(a[7]), &kc = tensor(a[8]), &vc = tensor(a[9]);
+  Tensor qw = optional(a[3]), kw = optional(a[4]), ks = optional(a[10]), vs = optional(a[11]);
+  check_rows(op, q0, k0, "q, k and v");
+  check_rows(op, q0, v0, "q, k and v");
+  need(v0.size(1) == k0.size(1), "qk_norm_rope: k and v must have the same heads");
+  const bool fp32 = check_weights(op, qw, kw, q0);
+  const int64_t tokens = q0.size(0), dim = q0.size(2);
+  const float eps = (float)number(a[12]);
+  Rotation rot(op, a[5], a[6], a[13], a[14], tokens, dim);
+  need(is_index(slots0) && slots0.dim() == 1 && slots0.size(0) == tokens, "qk_norm_rope: slot_mapping must be int32 or int64 [tokens]");
+  const CacheArg kca(op, kc, ks, q0.scalar_type()), vca(op, vc, vs, q0.scalar_type());
+  need(kc.sizes() == vc.sizes() && kc.scalar_type() == vc.scalar_type() && kc.size(2) == k0.size(1) && kc.size(3) == dim && kc.size(1) >= 1,
+       "qk_norm_rope: caches must be [pages, page_size, k's heads, dim], of one type");
+  OneDevice dev(op, {&q0, &k0, &v0, &qw, &kw, &rot.positions, &rot.freq, &slots0, &kc, &vc, &ks, &vs});
+  const Tensor slots = dense(slots0);
+  HeadRows q(q0), k(k0), v(v0);
+  Tensor qo = empty(q0.sizes(), q0.scalar_type(), q0);
+  void *pp = rot.positions.data_ptr(), *fp = rot.freq.data_ptr(), *qp = qo.data_ptr(), *sp = slots.data_ptr(),
+       *qwp = qw.defined() ? qw.data_ptr() : nullptr, *kwp = kw.defined() ? kw.data_ptr() : nullptr, *st = current_stream();
+  const int dt = element(q0.scalar_type()), ct = element(kc.scalar_type()), wide = slots.scalar_type() == at::kLong;
+  const int64_t pages = kc.size(0), page_size = kc.size(1);
+  check_status(without_gil([&] {
+                 return ako4x_qk_norm_rope_cache(&q.r, &k.r, &v.r, qwp, kwp, fp32, eps, pp, rot.wide(), (const float*)fp, rot.rotary,
+                                                 rot.interleaved, rot.factor, qp, sp, wide, &kca.c, &vca.c, ct, pages, page_size,
+                                                 tokens, dim, dt, st);
+               }),
+               "ako4x_qk_norm_rope_cache");
+  return pack(std::move(qo));
+  END_HANDLE_TH_ERRORS
+}
+
+// (q, k_cache, v_cache, block_table, seq_lens, sm_scale, k_scale, v_scale, window)
+PyObject* paged_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const char* op = "paged_decode";
+  count(n, 9, op);
+  c10::NoGradGuard ng;
+  const Tensor &q0 = tensor(a[0]), &kc = tensor(a[1]), &vc = tensor(a[2]), &table0 = tensor(a[3]), &lens0 = tensor(a[4]),
+               ks = optional(a[6]), vs = optional(a[7]);
+  const float scale = (float)number(a[5]);
+  const int64_t window = a[8] == Py_None ? 0 : integer(a[8]);
+  need(q0.dim() == 3 && (q0.size(2) == 64 || q0.size(2) == 128 || q0.size(2) == 256), "paged_decode: q must be [batch, heads, 64, 128 or 256]");
+  need(q0.scalar_type() == at::kBFloat16 || q0.scalar_type() == at::kHalf, "paged_decode: q must be bf16 or fp16");
+  const CacheArg kca(op, kc, ks, q0.scalar_type()), vca(op, vc, vs, q0.scalar_type());
+  const int64_t batch = q0.size(0), hq = q0.size(1), dim = q0.size(2), pages = kc.size(0), page_size = kc.size(1), hk = kc.size(2);
+  need(vc.sizes() == kc.sizes() && vc.scalar_type() == kc.scalar_type() && kc.size(3) == dim && page_size >= 1,
+       "paged_decode: caches must be [pages, page_size, kv_heads, dim], of one type");
+  need(hq >= 1 && hk >= 1 && hq % hk == 0 && hq <= 65536, "paged_decode: q's heads must be a multiple of the caches'");
+  need(table0.scalar_type() == at::kInt && table0.dim() == 2 && table0.size(0) == batch && lens0.scalar_type() == at::kInt &&
+           lens0.dim() == 1 && lens0.size(0) == batch,
+       "paged_decode: block_table int32 [batch, max_pages], seq_lens int32 [batch]");
+  need(window >= 0, "paged_decode: window must be 0 (none) or a number of tokens");
+  OneDevice dev(op, {&q0, &kc, &vc, &table0, &lens0, &ks, &vs});
+  const Tensor q = dense(q0), table = dense(table0), lens = dense(lens0);
+  const int64_t max_pages = table.size(1);
+  Tensor o = empty(q.sizes(), q.scalar_type(), q), lse = empty({batch, hq}, at::kFloat, q);
+  Workspace ws(ako4x_paged_decode_workspace_bytes(batch, hq, hk, dim, max_pages, page_size, window), q);
+  void *qp = ptr(q), *tp = table.data_ptr(), *lp = lens.data_ptr(), *st = current_stream();
+  const int dt = element(q.scalar_type()), ct = element(kc.scalar_type());
+  check_status(without_gil([&] {
+                 return ako4x_paged_decode(qp, &kca.c, &vca.c, (const int32_t*)tp, (const int32_t*)lp, scale, window, o.data_ptr(),
+                                           (float*)lse.data_ptr(), batch, hq, hk, dim, pages, page_size, max_pages, dt, ct, ws.p,
+                                           ws.bytes, st);
+               }),
+               "ako4x_paged_decode");
+  return pack_tuple(std::move(o), std::move(lse));
+  END_HANDLE_TH_ERRORS
+}
+
+// ---- pages of a cache ----
+
+// The tensors that have pages along their first dimension.
+struct PagedTensors {
+  std::vector<Tensor> t;
+  std::vector<void*> data;
+  std::vector<int64_t> bytes, strides;
+  PagedTensors(const char* op, PyObject* list, int64_t pages) {   // pages < 0: those of the first one
+    PyObject* seq = PySequence_Fast(list, "caches: a list of tensors expected");
+    if (!seq) throw python_error();
+    try {
+      for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(seq); ++i) t.push_back(tensor(PySequence_Fast_GET_ITEM(seq, i)));
+    } catch (...) {
+      Py_DECREF(seq);
+      throw;
+    }
+    Py_DECREF(seq);
+    for (const Tensor& x : t) {
+      if (x.dim() >= 1 && pages < 0) pages = x.size(0);
+      if (x.dim() < 1 || x.size(0) != pages) fail(std::string(op) + ": every cache must have the pages along its first dimension");
+      if (x.numel() == 0) continue;
+      const int64_t per = x.numel() / pages;
+      if (!(x.select(0, 0).is_non_overlapping_and_dense() && (pages == 1 || x.stride(0) >= per)))
+        fail(std::string(op) + ": a page of a cache must be one piece of memory");
+      data.push_back(x.data_ptr());
+      bytes.push_back(per * (int64_t)x.element_size());
+      strides.push_back(pages == 1 ? bytes.back() : x.stride(0) * (int64_t)x.element_size());
+    }
+    num_pages = pages;
+  }
+  int64_t num_pages;
+  int64_t count() const { return (int64_t)data.size(); }
+};
+// The state, changed in place: block_table int32 [rows, max_pages], seq_lens int32 [rows], ref_counts int32 [pages].
+void check_state(const char* op, const Tensor& table, const Tensor* lens, const Tensor& refs) {
+  auto ok = [](const Tensor& t, int64_t dims) { return t.scalar_type() == at::kInt && t.dim() == dims && t.is_contiguous(); };
+  if (!(ok(table, 2) && (!lens || (ok(*lens, 1) && lens->size(0) == table.size(0))) && ok(refs, 1)))
+    fail(std::string(op) + ": block_table [rows, max_pages], seq_lens [rows] and ref_counts [pages] must be int32 and contiguous");
+}
+void check_list(const char* op, const char* what, const Tensor& a, const Tensor& b) {
+  if (!(a.scalar_type() == at::kInt && b.scalar_type() == at::kInt && a.dim() == 1 && b.dim() == 1 && a.size(0) == b.size(0)))
+    fail(std::string(op) + ": " + what + " must be int32 [n]");
+}
+int64_t page_size_of(const char* op, PyObject* o) {
+  const int64_t v = integer(o);
+  if (v < 1) fail(std::string(op) + ": page_size must be positive");
+  return v;
+}
+OneDevice device_of(const char* op, std::initializer_list<const Tensor*> all, const PagedTensors* caches) {
+  if (caches)
+    for (const Tensor& t : caches->t)
+      for (const Tensor* x : all)
+        if (t.is_cuda() && x->is_cuda() && t.device() != x->device()) fail(std::string(op) + ": tensors on different devices");
+  if (caches)
+    for (const Tensor& t : caches->t) need(t.is_cuda(), "ako4x_b200 operators take CUDA tensors only (there is no CPU path)");
+  return OneDevice(op, all);
+}
+
+// (caches, src, dst)
+PyObject* kv_pages_copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const char* op = "kv_pages.copy";
+  count(n, 3, op);
+  c10::NoGradGuard ng;
+  const Tensor &s0 = tensor(a[1]), &d0 = tensor(a[2]);
+  check_list(op, "src and dst", s0, d0);
+  const PagedTensors c(op, a[0], -1);
+  need(!c.t.empty(), "kv_pages.copy: no caches");
+  OneDevice dev = device_of(op, {&s0, &d0}, &c);
+  const Tensor src = dense(s0), dst = dense(d0);
+  const int64_t pairs = src.size(0);
+  Tensor ok = empty({1}, at::kBool, src);
+  Workspace ws(ako4x_kv_pages_copy_workspace_bytes(pairs, c.num_pages), src);
+  void *sp = src.data_ptr(), *dp = dst.data_ptr(), *op_ = ok.data_ptr(), *st = current_stream();
+  check_status(without_gil([&] {
+                 return ako4x_kv_pages_copy(c.data.data(), c.bytes.data(), c.strides.data(), c.count(), (const int32_t*)sp,
+                                            (const int32_t*)dp, (uint8_t*)op_, pairs, c.num_pages, ws.p, ws.bytes, st);
+               }),
+               "ako4x_kv_pages_copy");
+  return pack(std::move(ok));
+  END_HANDLE_TH_ERRORS
+}
+
+// (block_table, seq_lens, ref_counts, rows, add, page_size)
+PyObject* kv_pages_extend(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const char* op = "kv_pages.extend";
+  count(n, 6, op);
+  c10::NoGradGuard ng;
+  const Tensor &table = tensor(a[0]), &lens = tensor(a[1]), &refs = tensor(a[2]), &r0 = tensor(a[3]), &d0 = tensor(a[4]);
+  check_state(op, table, &lens, refs);
+  check_list(op, "rows and add", r0, d0);
+  const int64_t ps = page_size_of(op, a[5]);
+  OneDevice dev(op, {&table, &lens, &refs, &r0, &d0});
+  const Tensor rows = dense(r0), add = dense(d0);
+  const int64_t m = rows.size(0), nr = table.size(0), mp = table.size(1), np = refs.size(0);
+  Tensor ok = empty({m}, at::kBool, rows);
+  Workspace ws(ako4x_kv_pages_extend_workspace_bytes(m, nr, np), rows);
+  void *tp = table.data_ptr(), *lp = lens.data_ptr(), *rp = refs.data_ptr(), *xp = rows.data_ptr(), *ap = add.data_ptr(),
+       *op_ = ok.data_ptr(), *st = current_stream();
+  check_status(without_gil([&] {
+                 return ako4x_kv_pages_extend((int32_t*)tp, (int32_t*)lp, (int32_t*)rp, (const int32_t*)xp, (const int32_t*)ap,
+                                              (uint8_t*)op_, m, nr, mp, np, ps, ws.p, ws.bytes, st);
+               }),
+               "ako4x_kv_pages_extend");
+  return pack(std::move(ok));
+  END_HANDLE_TH_ERRORS
+}
+
+// (block_table, seq_lens, ref_counts, rows, page_size): returns None
+PyObject* kv_pages_free(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const char* op = "kv_pages.free";
+  count(n, 5, op);
+  c10::NoGradGuard ng;
+  const Tensor &table = tensor(a[0]), &lens = tensor(a[1]), &refs = tensor(a[2]), &r0 = tensor(a[3]);
+  check_state(op, table, &lens, refs);
+  check_list(op, "rows", r0, r0);
+  const int64_t ps = page_size_of(op, a[4]);
+  OneDevice dev(op, {&table, &lens, &refs, &r0});
+  const Tensor rows = dense(r0);
+  const int64_t m = rows.size(0), nr = table.size(0), mp = table.size(1), np = refs.size(0);
+  void *tp = table.data_ptr(), *lp = lens.data_ptr(), *rp = refs.data_ptr(), *xp = rows.data_ptr(), *st = current_stream();
+  check_status(without_gil([&] {
+                 return ako4x_kv_pages_free((int32_t*)tp, (int32_t*)lp, (int32_t*)rp, (const int32_t*)xp, m, nr, mp, np, ps, st);
+               }),
+               "ako4x_kv_pages_free");
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+// (caches, block_table, seq_lens, ref_counts, parents, children, page_size)
+PyObject* kv_pages_fork(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const char* op = "kv_pages.fork";
+  count(n, 7, op);
+  c10::NoGradGuard ng;
+  const Tensor &table = tensor(a[1]), &lens = tensor(a[2]), &refs = tensor(a[3]), &p0 = tensor(a[4]), &c0 = tensor(a[5]);
+  check_state(op, table, &lens, refs);
+  check_list(op, "parents and children", p0, c0);
+  const int64_t ps = page_size_of(op, a[6]);
+  const PagedTensors c(op, a[0], refs.size(0));
+  OneDevice dev = device_of(op, {&table, &lens, &refs, &p0, &c0}, &c);
+  const Tensor parents = dense(p0), children = dense(c0);
+  const int64_t m = parents.size(0), nr = table.size(0), mp = table.size(1), np = refs.size(0);
+  Tensor ok = empty({m}, at::kBool, parents);
+  Workspace ws(ako4x_kv_pages_fork_workspace_bytes(m, nr, np), parents);
+  void *tp = table.data_ptr(), *lp = lens.data_ptr(), *rp = refs.data_ptr(), *pp = parents.data_ptr(), *cp = children.data_ptr(),
+       *op_ = ok.data_ptr(), *st = current_stream();
+  check_status(without_gil([&] {
+                 return ako4x_kv_pages_fork(c.data.data(), c.bytes.data(), c.strides.data(), c.count(), (int32_t*)tp, (int32_t*)lp,
+                                            (int32_t*)rp, (const int32_t*)pp, (const int32_t*)cp, (uint8_t*)op_, m, nr, mp, np, ps,
+                                            ws.p, ws.bytes, st);
+               }),
+               "ako4x_kv_pages_fork");
+  return pack(std::move(ok));
+  END_HANDLE_TH_ERRORS
+}
+
+// (caches, block_table, ref_counts)
+PyObject* kv_pages_compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const char* op = "kv_pages.compact";
+  count(n, 3, op);
+  c10::NoGradGuard ng;
+  const Tensor &table = tensor(a[1]), &refs = tensor(a[2]);
+  check_state(op, table, nullptr, refs);
+  const PagedTensors c(op, a[0], refs.size(0));
+  OneDevice dev = device_of(op, {&table, &refs}, &c);
+  const int64_t nr = table.size(0), mp = table.size(1), np = refs.size(0);
+  Tensor map = empty({np}, at::kInt, refs);
+  Workspace ws(ako4x_kv_pages_compact_workspace_bytes(np), refs);
+  void *tp = table.data_ptr(), *rp = refs.data_ptr(), *mpp = map.data_ptr(), *st = current_stream();
+  check_status(without_gil([&] {
+                 return ako4x_kv_pages_compact(c.data.data(), c.bytes.data(), c.strides.data(), c.count(), (int32_t*)tp, (int32_t*)rp,
+                                               (int32_t*)mpp, nr, mp, np, ws.p, ws.bytes, st);
+               }),
+               "ako4x_kv_pages_compact");
+  return pack(std::move(map));
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef kMethods[] = {
 #define AKO_METHOD(f) {#f, (PyCFunction)(void (*)(void))f, METH_FASTCALL, nullptr}
     AKO_METHOD(rmsnorm),       AKO_METHOD(gqa_decode),  AKO_METHOD(mla_decode),
     AKO_METHOD(mla_prefill),   AKO_METHOD(dsa_indexer), AKO_METHOD(dsa_attention),
     AKO_METHOD(dsa_indexer_attention), AKO_METHOD(quantize_1x128), AKO_METHOD(index_k_cache_write),
     AKO_METHOD(moe),           AKO_METHOD(gdn_decode),  AKO_METHOD(gdn_prefill),
-    AKO_METHOD(gemm),          {nullptr, nullptr, 0, nullptr}};
+    AKO_METHOD(gemm),          AKO_METHOD(rope),        AKO_METHOD(qk_norm_rope),
+    AKO_METHOD(qk_norm_rope_cache), AKO_METHOD(paged_decode), AKO_METHOD(kv_pages_copy),
+    AKO_METHOD(kv_pages_extend), AKO_METHOD(kv_pages_free), AKO_METHOD(kv_pages_fork),
+    AKO_METHOD(kv_pages_compact), {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_native", "Native operator entry points.", -1, kMethods,
                        nullptr, nullptr, nullptr, nullptr};

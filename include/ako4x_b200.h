@@ -327,6 +327,118 @@ int ako4x_gdn_prefill(const void* q, const void* k, const void* v, const float* 
                       int64_t total_tokens, int64_t num_seqs, void* workspace,
                       size_t workspace_bytes, void* stream);
 
+/* ---- New tokens into and through a paged cache (no counterpart in the reference) ----------------
+ * Element types of these entry points. */
+#define AKO4X_BF16 0
+#define AKO4X_FP16 1
+#define AKO4X_E4M3 2
+
+/* Heads of every token, [tokens, heads, dim] with the last dimension contiguous: a view, for instance, of
+ * one projection's output. Strides in elements; data and strides are multiples of 16 bytes. */
+typedef struct {
+  const void* data;
+  int64_t token_stride, head_stride;
+  int64_t heads;
+} ako4x_head_rows;
+
+/* Keys (or values) of a paged cache, [num_pages, page_size, heads, dim] with the last dimension contiguous
+ * and any strides (in elements; data and strides multiples of 16 bytes): pages of whole tokens, pages of whole
+ * heads, keys and values side by side. In an e4m3 cache the value of an element is e4m3 * scale, with
+ * one fp32 scale per slot and head, [num_pages, page_size, heads] of strides of its own; otherwise NULL. */
+typedef struct {
+  void* data;
+  float* scale;
+  int64_t page_stride, slot_stride, head_stride;
+  int64_t scale_page_stride, scale_slot_stride, scale_head_stride;
+} ako4x_kv_cache;
+
+/* Rotary positions. The first rotary_dim (even, <= dim) elements of each head are rotated in pairs, (i, i +
+ * rotary_dim / 2) or, interleaved, (2i, 2i + 1), by the angle position * inv_freq[i]; cosine and sine are
+ * multiplied by attention_factor (scalings for long contexts); the other elements are copied. Angles in fp64,
+ * the rest in fp32, rounded once. q, k bf16 or fp16 (`dtype`), dim a multiple of 8 up to 256; k may be NULL;
+ * positions int32 or int64 [tokens]; inv_freq fp32 [rotary_dim / 2]; q_out, k_out [tokens, heads, dim]
+ * contiguous, not overlapping the inputs. One launch, no workspace. */
+int ako4x_rope(const ako4x_head_rows* q, const ako4x_head_rows* k, const void* positions, int positions_int64,
+               const float* inv_freq, int64_t rotary_dim, int interleaved, float attention_factor, void* q_out,
+               void* k_out, int64_t tokens, int64_t dim, int dtype, void* stream);
+/* The same behind an RMS norm of every head in the same pass: x * rsqrt(mean(x^2) + eps) * weight over
+ * dim; weights of the rows' type or fp32, [dim]. */
+int ako4x_qk_norm_rope(const ako4x_head_rows* q, const ako4x_head_rows* k, const void* q_weight,
+                       const void* k_weight, int weights_fp32, float eps, const void* positions, int positions_int64,
+                       const float* inv_freq, int64_t rotary_dim, int interleaved, float attention_factor,
+                       void* q_out, void* k_out, int64_t tokens, int64_t dim, int dtype, void* stream);
+/* The same with the keys, and the values as they are, stored into a paged cache at slot_mapping[token] = page *
+ * page_size + slot (int32 or int64, distinct; a token whose slot is negative or past the cache is not stored, its
+ * query is computed all the same). A NULL weight leaves that norm out. The cache is of the rows' type, or e4m3: then
+ * each row gets scale = amax / 448 (1 when amax <= 1e-10, NaN for a row with a NaN), values e4m3(x / scale) from
+ * the fp32 x. */
+int ako4x_qk_norm_rope_cache(const ako4x_head_rows* q, const ako4x_head_rows* k, const ako4x_head_rows* v,
+                             const void* q_weight, const void* k_weight, int weights_fp32, float eps,
+                             const void* positions, int positions_int64, const float* inv_freq, int64_t rotary_dim,
+                             int interleaved, float attention_factor, void* q_out, const void* slot_mapping,
+                             int slots_int64, const ako4x_kv_cache* k_cache, const ako4x_kv_cache* v_cache,
+                             int cache_dtype, int64_t num_pages, int64_t page_size, int64_t tokens, int64_t dim,
+                             int dtype, void* stream);
+
+/* Attention of one new token per sequence over a paged cache read through a block table. q [batch, q_heads, dim]
+ * contiguous, bf16 or fp16; caches of q's type or e4m3; dim 64, 128 or 256; q_heads a multiple of kv_heads, query
+ * head h reads KV head h / (q_heads / kv_heads). Token t of sequence b lies in page block_table[b, t / page_size],
+ * slot t % page_size; seq_lens[b] tokens (at most max_pages * page_size are read), of which the last `window` are
+ * visible (0: all). Tokens of a page id outside [0, num_pages) are not visible. o like q, lse fp32 [batch,
+ * q_heads] = log2(sum exp(sm_scale q.k)); a sequence that sees nothing gives o = 0, lse = -inf. */
+size_t ako4x_paged_decode_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim,
+                                          int64_t max_pages, int64_t page_size, int64_t window);
+int ako4x_paged_decode(const void* q, const ako4x_kv_cache* k_cache, const ako4x_kv_cache* v_cache,
+                       const int32_t* block_table, const int32_t* seq_lens, float sm_scale, int64_t window, void* o,
+                       float* lse, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t num_pages,
+                       int64_t page_size, int64_t max_pages, int dtype, int cache_dtype, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* The pages of a cache. What is kept: block_table int32 [rows, max_pages] (the pages of a row's tokens in order, -1
+ * behind them), seq_lens int32 [rows], ref_counts int32 [num_pages] (how many table entries name the page; 0: it is
+ * free). Fresh pages are the lowest free ones, handed out in the order of the request. A page that is not full
+ * belongs to one row. Requests are int32 device arrays of n entries; one that cannot be met changes nothing and
+ * gets ok = 0 (ok: one byte each). Nothing out of range is ever read or written: a row outside [0, rows) is
+ * not ok, a page id outside [0, num_pages) is passed over.
+ *
+ * extend: row rows[i] grows by add[i] >= 0 tokens (slots without contents). Not ok: a row listed before, more
+ * than max_pages, or no pages left for it (pages are set aside in the order of the request, whether or not the
+ * requests before were met). */
+size_t ako4x_kv_pages_extend_workspace_bytes(int64_t n, int64_t num_rows, int64_t num_pages);
+int ako4x_kv_pages_extend(int32_t* block_table, int32_t* seq_lens, int32_t* ref_counts, const int32_t* rows,
+                          const int32_t* add, uint8_t* ok, int64_t n, int64_t num_rows, int64_t max_pages,
+                          int64_t num_pages, int64_t page_size, void* workspace, size_t workspace_bytes,
+                          void* stream);
+/* free: the rows are emptied and their pages given back; empty rows, and rows listed twice, are fine. */
+int ako4x_kv_pages_free(int32_t* block_table, int32_t* seq_lens, int32_t* ref_counts, const int32_t* rows, int64_t n,
+                        int64_t num_rows, int64_t max_pages, int64_t num_pages, int64_t page_size, void* stream);
+/* Contents: `caches` (host array of num_caches) are the tensors that have a page of page_bytes[c] bytes at
+ * caches[c] + page * page_strides[c] (bytes), keys and values of every layer, scales and all.
+ *
+ * fork: the empty row children[i] becomes a copy of row parents[i] as it was before the call: full pages are shared,
+ * the last one, if it is not full, is copied to a fresh page. Not ok: a child that is not empty or listed before, or
+ * no page left. */
+size_t ako4x_kv_pages_fork_workspace_bytes(int64_t n, int64_t num_rows, int64_t num_pages);
+int ako4x_kv_pages_fork(void* const* caches, const int64_t* page_bytes, const int64_t* page_strides, int64_t num_caches,
+                        int32_t* block_table, int32_t* seq_lens, int32_t* ref_counts, const int32_t* parents,
+                        const int32_t* children, uint8_t* ok, int64_t n, int64_t num_rows, int64_t max_pages,
+                        int64_t num_pages, int64_t page_size, void* workspace, size_t workspace_bytes, void* stream);
+/* copy: page src[i] to page dst[i] in every cache. Pairs with an id out of range, and src = dst, are passed over. A
+ * list in which a page is the destination of two pairs, or the destination of one and the source of another,
+ * is refused on the device: nothing is copied, ok[0] = 0. */
+size_t ako4x_kv_pages_copy_workspace_bytes(int64_t n, int64_t num_pages);
+int ako4x_kv_pages_copy(void* const* caches, const int64_t* page_bytes, const int64_t* page_strides, int64_t num_caches,
+                        const int32_t* src, const int32_t* dst, uint8_t* ok, int64_t n, int64_t num_pages,
+                        void* workspace, size_t workspace_bytes, void* stream);
+/* compact: the u pages in use move into the first u places: the highest one in use into the lowest free place and
+ * so on, pages below u stay. Contents, block_table and ref_counts follow; page_map int32 [num_pages] is every
+ * page's new place, -1 for the free ones. */
+size_t ako4x_kv_pages_compact_workspace_bytes(int64_t num_pages);
+int ako4x_kv_pages_compact(void* const* caches, const int64_t* page_bytes, const int64_t* page_strides,
+                           int64_t num_caches, int32_t* block_table, int32_t* ref_counts, int32_t* page_map,
+                           int64_t num_rows, int64_t max_pages, int64_t num_pages, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -12,3 +12,4 @@ from .moe import ds_routing, moe_fp8_block_scale  # noqa: F401
 from .quantize import fp8_quantize_1x128, index_k_cache_write  # noqa: F401
 from .gdn import gdn_decode, gdn_prefill  # noqa: F401
 from .gemm import gemm_nt  # noqa: F401
+from . import paged  # noqa: F401
