@@ -8,13 +8,19 @@
 // Everything between the load and the one rounding of the result is fp32, but the angles: pos f_i has as
 // many digits in front of the point as the position, so the product is taken in fp64, in turns
 // (f_i / 2 pi), and its whole quarter turns are taken off there; what is left fits an fp32 sincospi to
-// its last bits, for any position. In the norm the factors of a token are the same for all its heads: z = (inv x) A + (inv x') B
-// with x' the partner and A = w c, B = -+ w' s kept in registers, 16 per lane.
+// its last bits, for any position. In the norm the factors of a token are the same for all its heads: z = inv (x A + x' B)
+// with x' the partner and A = w c, B = -+ w' s kept in registers.
 //
-// HBM-bound: every element is read and written once. 8, 16 or 32 lanes own a row (16 bytes each), a warp
-// takes row groups of one token (all of them, or a share where there are few tokens), four loads in flight
-// per lane; the token's R/2 angles are shared out over the lanes once. The partner is R/16 lanes away (one
-// shuffle per word), in the same lane (interleaved), or, where R/2 is no multiple of 8, read again.
+// HBM-bound: every element is read and written once. 4, 8 or 16 lanes own a row, two pieces of 16 bytes each,
+// and a lane's second piece holds the partners of its first: nothing is exchanged but the sum of the squares, and
+// nothing is unpacked twice. A warp takes row groups of one token (all of them, or a share where there are few
+// tokens), the loads two groups ahead; the token's R/2 angles are shared out over the lanes once.
+// Interleaved pairs lie in one piece; where R/2 is no multiple of 8 the partners are read again.
+// Measured, 8 192 tokens with 32 + 8 + 8 heads of 128 into a bf16 cache (201 MB): one piece per lane and partners by
+// shuffle 72 us; two pieces 61; grid without divisions, tables from whole vectors 51; loads ahead across the kinds of
+// rows, 20 warps to an SM 45 (4.5 TB/s). The same without arithmetic 31: what is left are instructions, 36 for a piece.
+#include <algorithm>
+
 #include "common.cuh"
 
 #include <cuda_fp16.h>
@@ -23,7 +29,6 @@ namespace {
 
 constexpr int WARPS = 4;
 constexpr int MAX_DIM = 256;
-constexpr int UNROLL = 4;
 
 struct Rows {                 // heads of one kind
   const unsigned char* in;
@@ -49,9 +54,9 @@ struct Params {
   Cache kc, vc;
   int64_t tokens, num_slots;
   int dim, rotary, page_size;
-  int shares;                 // warps per token
+  int per_share;              // groups of a warp
   float eps, inv_dim, factor;
-  bool interleaved, positions64, slots64, weights32, quant;
+  bool interleaved, positions64, slots64, weights32, quant, ragged;   // ragged: some lanes are behind the row's end
 };
 
 template <class T>
@@ -72,64 +77,81 @@ struct Pair<__half> {
   static __device__ __forceinline__ float one(const void* p) { return __half2float(*(const __half*)p); }
 };
 
-template <class T>
-__device__ __forceinline__ void unpack(const uint4& v, float (&x)[8]) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 p = Pair<T>::get(w[i]);
-    x[2 * i] = p.x;
-    x[2 * i + 1] = p.y;
-  }
-}
-template <class T>
-__device__ __forceinline__ uint4 packed(const float (&x)[8]) {
-  return make_uint4(Pair<T>::put(x[0], x[1]), Pair<T>::put(x[2], x[3]), Pair<T>::put(x[4], x[5]), Pair<T>::put(x[6], x[7]));
-}
+using F2 = float2;
+__device__ __forceinline__ F2 f2(float a, float b) { return make_float2(a, b); }
+__device__ __forceinline__ float2 both(F2 a) { return a; }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) { return make_float2(fmaf(a.x, b.x, c.x), fmaf(a.y, b.y, c.y)); }
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) { return make_float2(a.x * b.x, a.y * b.y); }
+
 __device__ __forceinline__ float max_nan(float a, float b) {   // a NaN stays
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-
-// 8 values of a row, quantised with the row's own scale: amax / 448, 1 for a row of (nearly) zeros.
-template <int LANES>
-__device__ __forceinline__ void store_e4m3(const float (&x)[8], unsigned char* to, float* scale, int lane, bool live) {
-  float top = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(x[i]));
-#pragma unroll
-  for (int o = LANES / 2; o >= 1; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float s = top <= 1e-10f ? 1.0f : __fdiv_rn(top, 448.0f);
-  if (!live) return;
-  uint32_t out[2] = {0u, 0u};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t pair = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(x[2 * i], s), __fdiv_rn(x[2 * i + 1], s)), __NV_SATFINITE, __NV_E4M3);
-    out[i >> 1] |= pair << (16 * (i & 1));
-  }
-  *(reinterpret_cast<uint2*>(to) + lane) = make_uint2(out[0], out[1]);
-  if (lane == 0) *scale = s;
-}
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
 // Where the partner of a rotated element is.
-enum Partner { OTHER_LANE, SAME_LANE, MEMORY };
+enum Partner { OTHER_PIECE, SAME_PIECE, MEMORY };
 
 template <class T, int LANES, Partner PARTNER>
-__global__ void __launch_bounds__(WARPS * 32) qk_norm_rope_kernel(const Params p) {
+__global__ void __launch_bounds__(WARPS * 32, PARTNER == MEMORY ? 3 : 5) qk_norm_rope_kernel(const Params p) {
   constexpr int GROUP = 32 / LANES;   // rows of a warp instruction
-  __shared__ float2 s_cs[WARPS][MAX_DIM / 2];
+  __shared__ __align__(16) float2 s_cs[WARPS][MAX_DIM / 2];
   const int warp = threadIdx.x >> 5, lane32 = threadIdx.x & 31;
   const int lane = lane32 % LANES, sub = lane32 / LANES;
-  const int64_t unit = (int64_t)blockIdx.x * WARPS + warp;
-  const int64_t token = unit / p.shares;
+  const int64_t token = (int64_t)blockIdx.x * WARPS + warp;
   if (token >= p.tokens) return;      // whole warps; there is no block barrier
-  const int share = (int)(unit - token * p.shares);
-  const int groups = p.q.groups + p.k.groups + p.v.groups;
-  const int g0 = (int)((int64_t)groups * share / p.shares), g1 = (int)((int64_t)groups * (share + 1) / p.shares);
+  const int end_q = p.q.groups, end_k = end_q + p.k.groups, end_v = end_k + p.v.groups;
+  const int g0 = blockIdx.y * p.per_share, g1 = min(g0 + p.per_share, end_v);
 
-  const int half = p.rotary / 2;
-  if (g0 < p.q.groups + p.k.groups) {
+  // this lane's two pieces of a row: the partners of each other in front, neighbours behind
+  const int half = p.rotary / 2, paired = PARTNER == OTHER_PIECE ? p.rotary / 16 : 0;
+  const int e0 = 8 * (lane < paired ? lane : 2 * lane), e1 = 8 * (lane < paired ? lane + paired : 2 * lane + 1);
+  const bool in0 = e0 < p.dim, in1 = e1 < p.dim;
+
+  // The loads run two row groups ahead, from one kind into the next. A lane past the last row, or past the row's
+  // end, reads what another one does.
+  int at = g0, at_kind = g0 < end_q ? 0 : g0 < end_k ? 1 : 2, at_stop, at_head, at_heads;
+  const unsigned char *from0, *from1;
+  int64_t step;
+  uint4 raw[2][2];
+  auto aim = [&] {
+    const Rows& r = at_kind == 0 ? p.q : at_kind == 1 ? p.k : p.v;
+    const int start = at_kind == 0 ? 0 : at_kind == 1 ? end_q : end_k;
+    at_stop = min(g1, start + r.groups);
+    at_head = (at - start) * GROUP + sub;
+    at_heads = r.heads;
+    from0 = r.in + token * r.token_stride + min(at_head, at_heads - 1) * r.head_stride;
+    from1 = from0 + (in1 ? e1 * 2 : 0);
+    from0 += in0 ? e0 * 2 : 0;
+    step = GROUP * r.head_stride;
+  };
+  auto fetch = [&](uint4 (&x)[2]) {
+    if (at >= g1) return;
+    x[0] = __ldg(reinterpret_cast<const uint4*>(from0));
+    x[1] = __ldg(reinterpret_cast<const uint4*>(from1));
+    if (++at == at_stop) {
+      if (at < g1) {
+        at_kind = at < end_k ? 1 : 2;
+        aim();
+      }
+    } else {
+      at_head += GROUP;
+      if (at_head < at_heads) {
+        from0 += step;
+        from1 += step;
+      }
+    }
+  };
+  aim();
+  fetch(raw[0]);                      // under way while the angles are made
+  fetch(raw[1]);
+  auto next = [&] {                   // called when raw[0] has been taken
+    raw[0][0] = raw[1][0], raw[0][1] = raw[1][1];
+    fetch(raw[1]);
+  };
+
+  if (g0 < end_k) {
     const double pos = p.positions64 ? (double)((const int64_t*)p.positions)[token] : (double)((const int32_t*)p.positions)[token];
     for (int i = lane32; i < half; i += 32) {
       double turn = pos * ((double)__ldg(p.inv_freq + i) * 0.15915494309189533577);   // f / 2 pi
@@ -144,123 +166,257 @@ __global__ void __launch_bounds__(WARPS * 32) qk_norm_rope_kernel(const Params p
     }
     __syncwarp();
   }
-  int64_t page = 0, slot = 0;
+  int64_t page = 0;
+  int slot = 0;
   bool stored = false;
   if (p.slots) {
     const int64_t at = p.slots64 ? ((const int64_t*)p.slots)[token] : (int64_t)((const int32_t*)p.slots)[token];
     stored = at >= 0 && at < p.num_slots;   // anything else: a padding token, its keys and values go nowhere
-    page = stored ? at / p.page_size : 0;
-    slot = stored ? at - page * p.page_size : 0;
+    if (stored) {
+      page = p.num_slots <= 0xffffffffLL ? (int64_t)((unsigned)at / (unsigned)p.page_size) : at / p.page_size;
+      slot = (int)(at - page * p.page_size);
+    }
   }
-  const int e0 = lane * 8;
-  const bool in_row = e0 < p.dim;
 
-  int first = 0;                       // groups in front of this kind
-#pragma unroll 1
-  for (int kind = 0; kind < 3; ++kind) {
-    const Rows& r = kind == 0 ? p.q : kind == 1 ? p.k : p.v;
-    const int lo = max(g0, first) - first, hi = min(g1, first + r.groups) - first;
-    first += r.groups;
-    if (lo >= hi) continue;
-    const bool to_cache = kind == 2 || (kind == 1 && !p.k_out);
-    if (to_cache && !stored) continue;
-    const void* weight = kind == 0 ? p.q_weight : kind == 1 ? p.k_weight : nullptr;
-    const bool turn = kind != 2;
-
-    // z = (inv x) A + (inv x') B
-    float A[8], B[8];
-    bool whole = turn;                 // all eight elements have a partner
+  // Pairs (2i, 2i + 1) of the pieces' elements: z = inv (x A + x' B), where `mask` says so; inv x A elsewhere.
+  F2 A[2][4], B[2][4];
+  unsigned mask = 0;
+  auto tables = [&](const void* weight) {
+    float w[2][8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      A[j] = 1.f;
-      B[j] = 0.f;
-      const int e = e0 + j;
-      const bool rot = turn && e < p.rotary;
-      whole &= rot;
-      int other = e, i = 0;
-      bool second = false;
-      if (rot) {
-        second = PARTNER == SAME_LANE ? (e & 1) : e >= half;
-        i = PARTNER == SAME_LANE ? e >> 1 : second ? e - half : e;
-        other = PARTNER == SAME_LANE ? e ^ 1 : second ? e - half : e + half;
-        const float2 cs = s_cs[warp][i];
-        A[j] = cs.x;
-        B[j] = second ? cs.y : -cs.y;
+    for (int h = 0; h < 2; ++h) {
+      const int e = h ? e1 : e0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[h][j] = 1.f;
+      if (weight && (h ? in1 : in0)) {
+        if (p.weights32) {
+#pragma unroll
+          for (int j = 0; j < 8; j += 4) {
+            const float4 y = __ldg(reinterpret_cast<const float4*>((const float*)weight + e + j));
+            w[h][j] = y.x, w[h][j + 1] = y.y, w[h][j + 2] = y.z, w[h][j + 3] = y.w;
+          }
+        } else {
+          const uint4 x = __ldg(reinterpret_cast<const uint4*>((const T*)weight + e));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 y = Pair<T>::get(word(x, j));
+            w[h][2 * j] = y.x;
+            w[h][2 * j + 1] = y.y;
+          }
+        }
       }
-      if (weight && in_row) {
-        A[j] *= p.weights32 ? __ldg((const float*)weight + e) : Pair<T>::one((const T*)weight + e);
-        if (rot) B[j] *= p.weights32 ? __ldg((const float*)weight + other) : Pair<T>::one((const T*)weight + other);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        A[h][j] = f2(w[h][2 * j], w[h][2 * j + 1]);
+        B[h][j] = f2(0.f, 0.f);
       }
     }
-    const int away = e0 < half ? half / 8 : -(half / 8);   // lanes to the partner
-
-    const unsigned char* base = r.in + token * r.token_stride + e0 * 2;
-#pragma unroll 1
-    for (int g = lo; g < hi; g += UNROLL) {
-      uint4 raw[UNROLL];
+    mask = 0;
+    if (PARTNER == OTHER_PIECE) {
+      if (lane < paired) {            // eight angles, of both pieces
+        mask = 0xffu;
 #pragma unroll
-      for (int u = 0; u < UNROLL; ++u) {
-        const int head = (g + u) * GROUP + sub;
-        raw[u] = make_uint4(0u, 0u, 0u, 0u);
-        if (g + u < hi && head < r.heads && in_row) raw[u] = __ldg(reinterpret_cast<const uint4*>(base + head * r.head_stride));
+        for (int j = 0; j < 4; ++j) {
+          const float4 cs = *reinterpret_cast<const float4*>(&s_cs[warp][e0 + 2 * j]);
+          A[0][j] = f2(w[0][2 * j] * cs.x, w[0][2 * j + 1] * cs.z);
+          A[1][j] = f2(w[1][2 * j] * cs.x, w[1][2 * j + 1] * cs.z);
+          B[0][j] = f2(-w[1][2 * j] * cs.y, -w[1][2 * j + 1] * cs.w);
+          B[1][j] = f2(w[0][2 * j] * cs.y, w[0][2 * j + 1] * cs.w);
+        }
       }
+    } else if (PARTNER == SAME_PIECE) {
 #pragma unroll
-      for (int u = 0; u < UNROLL; ++u) {
-        if (g + u >= hi) break;        // the whole warp
-        const int head = (g + u) * GROUP + sub;
-        const bool live = head < r.heads && in_row;
-        float x[8], y[8];
-        unpack<T>(raw[u], x);
-        if (turn) {
-          float o[8];                  // the partners
-          if (PARTNER == OTHER_LANE) {
-            const int from = lane32 + away;
-            const uint4 w = make_uint4(__shfl_sync(0xffffffffu, raw[u].x, from), __shfl_sync(0xffffffffu, raw[u].y, from),
-                                       __shfl_sync(0xffffffffu, raw[u].z, from), __shfl_sync(0xffffffffu, raw[u].w, from));
-            unpack<T>(w, o);
-          } else if (PARTNER == SAME_LANE) {
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) o[j] = x[j ^ 1];
-          } else {
+        for (int j = 0; j < 4; ++j) {
+          const int e = (h ? e1 : e0) + 2 * j;
+          if (e < p.rotary) {
+            const float2 cs = s_cs[warp][e / 2];
+            mask |= 1u << (4 * h + j);
+            A[h][j] = f2(w[h][2 * j] * cs.x, w[h][2 * j + 1] * cs.x);
+            B[h][j] = f2(-w[h][2 * j + 1] * cs.y, w[h][2 * j] * cs.y);
+          }
+        }
+    } else {                          // the partner's weight is met where the partner is read
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const int e = e0 + j;
-              o[j] = 0.f;
-              if (live && e < p.rotary)
-                o[j] = Pair<T>::one(base + head * r.head_stride + (j + (e < half ? half : -half)) * 2);
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float a[2] = {w[h][2 * j], w[h][2 * j + 1]}, b[2] = {0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int e = (h ? e1 : e0) + 2 * j + c;
+            if (e < p.rotary) {
+              const float2 cs = s_cs[warp][e < half ? e : e - half];
+              a[c] *= cs.x;
+              b[c] = e < half ? -cs.y : cs.y;
             }
           }
-          if (!whole) {                // an element that is not rotated takes nothing from another one
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (e0 + j >= p.rotary) o[j] = 0.f;
-          }
-          float inv = 1.f;
-          if (weight) {
-            float ss = 0.f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
-#pragma unroll
-            for (int m = LANES / 2; m >= 1; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-            inv = rsqrtf(fmaf(ss, p.inv_dim, p.eps));
-          }
-#pragma unroll
-          for (int j = 0; j < 8; ++j) y[j] = fmaf(x[j] * inv, A[j], (o[j] * inv) * B[j]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) y[j] = x[j];
+          A[h][j] = f2(a[0], a[1]);
+          B[h][j] = f2(b[0], b[1]);
         }
-        if (!to_cache) {
-          unsigned char* out = kind == 0 ? p.q_out : p.k_out;
-          if (live) __stcs(reinterpret_cast<uint4*>(out + ((token * r.heads + head) * p.dim + e0) * 2), packed<T>(y));
-        } else {
-          const Cache& c = kind == 1 ? p.kc : p.vc;
-          unsigned char* to = c.data + page * c.page_stride + slot * c.slot_stride + head * c.head_stride;
-          if (p.quant)
-            store_e4m3<LANES>(y, to, c.scale + page * c.scale_page_stride + slot * c.scale_slot_stride + head * c.scale_head_stride,
-                              lane, live);
-          else if (live)
-            *(reinterpret_cast<uint4*>(to) + lane) = packed<T>(y);
+    }
+  };
+
+  const bool all = PARTNER != MEMORY && p.rotary == p.dim;   // every element is rotated
+  bool ready = false;
+#pragma unroll 1
+  for (int it = g0; it < g1;) {       // a kind
+    const int kind = it < end_q ? 0 : it < end_k ? 1 : 2, start = kind == 0 ? 0 : kind == 1 ? end_q : end_k;
+    const Rows& r = kind == 0 ? p.q : kind == 1 ? p.k : p.v;
+    const int heads = r.heads, stop = min(g1, start + r.groups);
+    int head = (it - start) * GROUP + sub;
+    const bool to_cache = kind == 2 || (kind == 1 && !p.k_out), turn = kind != 2;
+    const void* weight = kind == 0 ? p.q_weight : kind == 1 ? p.k_weight : nullptr;
+    if (turn && (weight || !ready)) {
+      tables(weight);
+      ready = weight == nullptr;
+    }
+    unsigned char* out;
+    int64_t out_step;
+    float* scale_out = nullptr;
+    int64_t scale_step = 0;
+    const bool quant = to_cache && p.quant;
+    if (!to_cache) {
+      out = (kind == 0 ? p.q_out : p.k_out) + (token * heads + head) * p.dim * 2;
+      out_step = (int64_t)GROUP * p.dim * 2;
+    } else {
+      const Cache& c = kind == 1 ? p.kc : p.vc;
+      out = c.data + page * c.page_stride + slot * c.slot_stride + head * c.head_stride;
+      out_step = GROUP * c.head_stride;
+      if (quant) {
+        scale_out = c.scale + page * c.scale_page_stride + slot * c.scale_slot_stride + head * c.scale_head_stride;
+        scale_step = GROUP * c.scale_head_stride;
+      }
+    }
+    unsigned char *to0 = out + (quant ? e0 : e0 * 2), *to1 = out + (quant ? e1 : e1 * 2);
+    const bool store = !to_cache || stored;
+    if (!turn && !quant) {            // values as they are
+#pragma unroll 1
+      for (; it < stop; ++it, head += GROUP, to0 += out_step, to1 += out_step) {
+        const uint4 x0 = raw[0][0], x1 = raw[0][1];
+        next();
+        if (store && head < heads && in0) __stcs(reinterpret_cast<uint4*>(to0), x0);
+        if (store && head < heads && in1) __stcs(reinterpret_cast<uint4*>(to1), x1);
+      }
+    }
+#pragma unroll 1
+    for (; it < stop; ++it, head += GROUP, to0 += out_step, to1 += out_step) {
+      const bool live = store && head < heads;
+      F2 y[2][4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 x = Pair<T>::get(word(raw[0][h], j));
+          y[h][j] = f2(x.x, x.y);
+        }
+      const unsigned char* row = PARTNER == MEMORY ? r.in + token * r.token_stride + min(head, heads - 1) * r.head_stride : nullptr;
+      next();
+      if (p.ragged) {                 // pieces behind the row's end
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (!(h ? in1 : in0)) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[h][j] = f2(0.f, 0.f);
+          }
+      }
+      if (turn) {
+        F2 o[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (PARTNER == OTHER_PIECE) {
+              o[h][j] = y[1 - h][j];
+            } else if (PARTNER == SAME_PIECE) {
+              const float2 x = both(y[h][j]);
+              o[h][j] = f2(x.y, x.x);
+            } else {
+              float v[2];
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                const int e = (h ? e1 : e0) + 2 * j + c, other = e < half ? e + half : e - half;
+                v[c] = 0.f;
+                if (e < p.rotary) {
+                  v[c] = Pair<T>::one(row + other * 2);
+                  if (weight) v[c] *= p.weights32 ? __ldg((const float*)weight + other) : Pair<T>::one((const T*)weight + other);
+                }
+              }
+              o[h][j] = f2(v[0], v[1]);
+            }
+          }
+        float inv = 1.f;
+        if (weight) {
+          F2 ss = mul2(y[0][0], y[0][0]), st = mul2(y[1][0], y[1][0]);
+#pragma unroll
+          for (int j = 1; j < 4; ++j) {
+            ss = fma2(y[0][j], y[0][j], ss);
+            st = fma2(y[1][j], y[1][j], st);
+          }
+          const float2 a = both(ss), b = both(st);
+          float sum = (a.x + a.y) + (b.x + b.y);
+#pragma unroll
+          for (int m = LANES / 2; m >= 1; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+          inv = rsqrtf(fmaf(sum, p.inv_dim, p.eps));
+        }
+        F2 z[2][4];
+        if (all || PARTNER == MEMORY) {   // MEMORY: the partner of an element that is not rotated is 0
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) z[h][j] = fma2(o[h][j], B[h][j], mul2(y[h][j], A[h][j]));
+        } else {                          // an element that is not rotated takes nothing from another one
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              z[h][j] = mul2(y[h][j], A[h][j]);
+              if (mask >> (4 * h + j) & 1) z[h][j] = fma2(o[h][j], B[h][j], z[h][j]);
+            }
+        }
+        const F2 by = f2(inv, inv);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) y[h][j] = weight ? mul2(z[h][j], by) : z[h][j];
+      }
+      if (quant) {
+        // e4m3 with the row's own scale: amax / 448, 1 for a row of (nearly) zeros
+        float top = 0.f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 x = both(y[h][j]);
+            top = max_nan(top, max_nan(fabsf(x.x), fabsf(x.y)));
+          }
+#pragma unroll
+        for (int m = LANES / 2; m >= 1; m >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, m));
+        const float sc = top <= 1e-10f ? 1.0f : __fdiv_rn(top, 448.0f);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t w[2] = {0u, 0u};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 x = both(y[h][j]);
+            const uint32_t pair = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(x.x, sc), __fdiv_rn(x.y, sc)), __NV_SATFINITE, __NV_E4M3);
+            w[j >> 1] |= pair << (16 * (j & 1));
+          }
+          if (live && (h ? in1 : in0)) *reinterpret_cast<uint2*>(h ? to1 : to0) = make_uint2(w[0], w[1]);
+        }
+        if (live && lane == 0) *scale_out = sc;
+        scale_out += scale_step;
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 x = both(y[h][j]);
+            w[j] = Pair<T>::put(x.x, x.y);
+          }
+          if (live && (h ? in1 : in0)) __stcs(reinterpret_cast<uint4*>(h ? to1 : to0), make_uint4(w[0], w[1], w[2], w[3]));
         }
       }
     }
@@ -268,19 +424,19 @@ __global__ void __launch_bounds__(WARPS * 32) qk_norm_rope_kernel(const Params p
 }
 
 template <class T, int LANES>
-void launch(const Params& p, unsigned blocks, cudaStream_t st) {
+void launch(const Params& p, dim3 blocks, cudaStream_t st) {
   if (p.interleaved)
-    qk_norm_rope_kernel<T, LANES, SAME_LANE><<<blocks, WARPS * 32, 0, st>>>(p);
+    qk_norm_rope_kernel<T, LANES, SAME_PIECE><<<blocks, WARPS * 32, 0, st>>>(p);
   else if (p.rotary % 16 == 0)
-    qk_norm_rope_kernel<T, LANES, OTHER_LANE><<<blocks, WARPS * 32, 0, st>>>(p);
+    qk_norm_rope_kernel<T, LANES, OTHER_PIECE><<<blocks, WARPS * 32, 0, st>>>(p);
   else
     qk_norm_rope_kernel<T, LANES, MEMORY><<<blocks, WARPS * 32, 0, st>>>(p);
 }
 template <class T>
-void launch(const Params& p, int lanes, unsigned blocks, cudaStream_t st) {
-  if (lanes == 8) launch<T, 8>(p, blocks, st);
-  else if (lanes == 16) launch<T, 16>(p, blocks, st);
-  else launch<T, 32>(p, blocks, st);
+void launch(const Params& p, int lanes, dim3 blocks, cudaStream_t st) {
+  if (lanes == 4) launch<T, 4>(p, blocks, st);
+  else if (lanes == 8) launch<T, 8>(p, blocks, st);
+  else launch<T, 16>(p, blocks, st);
 }
 
 bool aligned(const void* ptr, int64_t a, int64_t b, int64_t c, int64_t to) {
@@ -292,7 +448,7 @@ int run(Params& p, const ako4x_head_rows* q, const ako4x_head_rows* k, const ako
   if (tokens < 0 || dim < 0 || rotary < 0) return AKO4X_EINVAL;
   if (dim < 8 || dim > MAX_DIM || dim % 8 || rotary > dim || rotary % 2) return AKO4X_EUNSUPPORTED_SHAPE;
   if (dtype != AKO4X_BF16 && dtype != AKO4X_FP16) return AKO4X_EUNSUPPORTED_SHAPE;
-  const int lanes = dim <= 64 ? 8 : dim <= 128 ? 16 : 32;
+  const int lanes = dim <= 64 ? 4 : dim <= 128 ? 8 : 16;
   const int group = 32 / lanes;
   const ako4x_head_rows* in[3] = {q, k, v};
   Rows* to[3] = {&p.q, &p.k, &p.v};
@@ -317,16 +473,18 @@ int run(Params& p, const ako4x_head_rows* q, const ako4x_head_rows* k, const ako
   p.dim = (int)dim;
   p.rotary = (int)rotary;
   p.inv_dim = 1.0f / (float)dim;
+  p.ragged = dim != lanes * 16;
   // A warp takes a token's rows, or a share of them while there are fewer warps than the GPU holds.
   const int64_t wanted = (int64_t)ako::sm_count() * 32;
-  int64_t shares = ako::cdiv(wanted, tokens);
-  if (shares > groups) shares = groups;
-  p.shares = (int)shares;
-  const int64_t blocks = ako::cdiv(tokens * shares, WARPS);
-  if (blocks > 0x7fffffffLL) return AKO4X_ETOOLARGE;
+  int64_t shares = std::min(ako::cdiv(wanted, tokens), groups);
+  p.per_share = (int)ako::cdiv(groups, shares);
+  shares = ako::cdiv(groups, (int64_t)p.per_share);
+  const int64_t blocks = ako::cdiv(tokens, (int64_t)WARPS);
+  if (blocks > 0x7fffffffLL || shares > 65535 || groups > 0x3fffffffLL) return AKO4X_ETOOLARGE;
+  const dim3 grid((unsigned)blocks, (unsigned)shares);
   cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == AKO4X_BF16) launch<__nv_bfloat16>(p, lanes, (unsigned)blocks, st);
-  else launch<__half>(p, lanes, (unsigned)blocks, st);
+  if (dtype == AKO4X_BF16) launch<__nv_bfloat16>(p, lanes, grid, st);
+  else launch<__half>(p, lanes, grid, st);
   AKO_CHECK_LAUNCH();
   return AKO4X_OK;
 }
