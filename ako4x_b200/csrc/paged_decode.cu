@@ -1,787 +1,18 @@
-// Attention of one new token per sequence over a paged cache: any number of query heads per KV head, head
-// sizes 64, 128 and 256, bf16 or fp16, caches of that type or e4m3 with a scale per slot and head, a block
-// table, and a sliding window.
-//
-//   s_t = scale q.k_t,  p_t = exp(s_t - m),  o = sum p_t v_t / sum p_t,  lse = m + log sum p_t
-//
-// in one pass over the keys with the running maximum m, in fp32 from the products on.
-//
-// HBM-bound: a key and its value are read once and met by the few query heads that share them, so nothing is
-// staged: a warp owns one KV head (eight of its query heads) and loads its keys straight into the operand
-// registers of mma.m16n8k16, tokens as M. Lane (g, t) has the 16-byte pieces t + 4 j of tokens g and g + 8;
-// the order of the reduction that this makes is given to q as well. V is loaded the same way and turned by
-// movmatrix, O^T = V^T P^T with features as M. There is no barrier and no shared memory in the loop; the
-// next tile's K is requested when S is computed, its V when O is.
-//   * P goes in as two pieces of 16 bits, both of them positive for a positive weight, so that an infinite
-//     value stays infinite: hi = P cut to its leading bits, lo = the rest. One piece would put its own rounding
-//     beside the output's, and more of it the fewer keys there are.
-//   * fp16: P is scaled by 2^15 on its way in (the sum too). A weight of 2^-24 of the largest is the
-//     smallest fp16 value otherwise, and a long tail of keys below it would vanish from o but not from lse.
-//   * e4m3 becomes fp16 exactly (one conversion for a pair: 1.6 cycles of an SM for the 128 values of a warp's word,
-//     against 3.6 by shifts to bf16). The scale of a key multiplies its score. The scale of a value multiplies
-//     its weight, over a power of two above all scales met so far, for fp16's range again.
-//
-// Work split: flat_share.cuh over tiles of 16 tokens. A CTA's warps take up to four (KV head, block of query heads)
-// pairs; where there are fewer, several warps take a pair's tiles in turn and put their parts together in shared
-// memory. A share that ends inside a sequence leaves a partial (m, l, O) for the merge kernel.
-#include <algorithm>
-#include <cfloat>
+// Paged decode: the entry points, and the kernels for bf16 queries.
+#include "paged_decode.cuh"
 
-#include <cuda_fp16.h>
-
-#include "flat_share.cuh"
+int ako::paged::run_bf16(const Params& p, const Plan& pl, int64_t dim, bool fp8, cudaStream_t st) {
+  return fp8 ? launch_dim<__nv_bfloat16, true>(p, pl, dim, st) : launch_dim<__nv_bfloat16, false>(p, pl, dim, st);
+}
 
 namespace {
 
-constexpr int TILE = 16;
+using namespace ako::paged;
 
-constexpr int WARPS = 4, THREADS = WARPS * 32;
-
-struct Cache {
-  const uint4* data;
-  const float* scale;
-  uint32_t page, slot, head;              // strides in 16 bytes
-  uint32_t scale_page, scale_slot, scale_head;   // in elements
-};
-struct Params {
-  const void* q;
-  Cache k, v;
-  const int32_t* table;
-  const int32_t* lens;
-  void* o;
-  float* lse;
-  float* part_acc;   // [slot][q_heads][D]
-  float* part_ml;    // [slot][q_heads][2]
-  int2* cut;
-  float scale_log2;
-  int batch, q_heads, kv_heads, group, head_blocks;   // head_blocks: warps for the query heads of a KV head
-  int per_cta, unit_ctas;   // (KV head, block) pairs of a CTA; CTAs of a share
-  int num_pages, page_size, page_shift, max_pages, window;
-  int shares;        // CTAs along the tiles
-  bool same_strides; // of K and V, scales too
-};
-
-// Entries for the merge, as in the split of the other decode kernels: {sequence, first share, shares}, one per
-// sequence where there are no more sequences than shares (a partial lies in slot sequence + share), otherwise one per
-// share, for the sequence that starts in it and goes on (slot 2 share, the first one of a sequence 2 share + 1).
-__device__ __forceinline__ int2 cut_entry(int b, int first, int n) { return make_int2(b, first | n << 16); }
-
-struct Span {          // visible tokens of a sequence
-  int lo, hi;
-  __device__ __forceinline__ int first_tile() const { return lo / TILE; }
-  __device__ __forceinline__ int tiles() const { return hi > lo ? (hi + TILE - 1) / TILE - lo / TILE : 0; }
-};
-__device__ __forceinline__ Span span_of(const Params& p, int b) {
-  const int64_t most = min((int64_t)p.max_pages * p.page_size, (int64_t)0x7fffff00);   // tiles end in 32 bits
-  Span s;
-  s.hi = p.num_pages > 0 ? (int)min((int64_t)max(0, p.lens[b]), most) : 0;
-  s.lo = p.window > 0 ? max(0, s.hi - p.window) : 0;
-  return s;
-}
-
-__device__ __forceinline__ uint4 ld16(const uint4* p) {
-  uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
-  return r;
-}
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ uint4 lds16(uint32_t a) {
-  uint4 r;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
-  return r;
-}
-__device__ __forceinline__ void lds_pair(uint32_t a, float& x, float& y) {
-  asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(x), "=f"(y) : "r"(a) : "memory");
-}
-__device__ __forceinline__ void sts16(uint32_t a, const uint4& v) {
-  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-}
-__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
-
-template <class T>
-__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
-template <>
-__device__ __forceinline__ void mma<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  ako::mma_bf16_16816(d, a, b0, b1);
-}
-template <>
-__device__ __forceinline__ void mma<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// The four e4m3 values of a word as two pairs of fp16: exact, NaN included.
-__device__ __forceinline__ void widen(uint32_t w, uint32_t& low, uint32_t& high) {
-  asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\ncvt.rn.f16x2.e4m3x2 %0, l;\ncvt.rn.f16x2.e4m3x2 %1, h;\n}\n"
-      : "=r"(low), "=r"(high)
-      : "r"(w));
-}
-__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }   // -126 .. 127
-// e with 2^e <= x < 2^(e + 1), within [-120, 120]
-__device__ __forceinline__ int exponent(float x) { return min(max(((int)(__float_as_uint(x) >> 23) & 0xff) - 127, -120), 120); }
-
-// A weight p >= 0 as hi + lo, both positive where p is.
-template <class T>
-__device__ __forceinline__ void two_pieces(float p0, float p1, uint32_t& hi, uint32_t& lo);
-template <>
-__device__ __forceinline__ void two_pieces<__nv_bfloat16>(float p0, float p1, uint32_t& hi, uint32_t& lo) {
-  hi = __byte_perm(__float_as_uint(p0), __float_as_uint(p1), 0x7632);   // cut
-  const float r0 = p0 - ako::bf16_lo(hi), r1 = p1 - ako::bf16_hi(hi);
-  lo = ako::pack_bf16x2(r0 == 0.f ? p0 * 0x1p-16f : r0, r1 == 0.f ? p1 * 0x1p-16f : r1);
-}
-template <>
-__device__ __forceinline__ void two_pieces<__half>(float p0, float p1, uint32_t& hi, uint32_t& lo) {
-  __half2 h = __halves2half2(__float2half_rz(p0), __float2half_rz(p1));
-  hi = *reinterpret_cast<uint32_t*>(&h);
-  const float2 c = __half22float2(h);
-  const float r0 = p0 > 0.f ? fmaxf(p0 - c.x, 0x1p-24f) : p0, r1 = p1 > 0.f ? fmaxf(p1 - c.y, 0x1p-24f) : p1;
-  __half2 l = __floats2half2_rn(r0, r1);
-  lo = *reinterpret_cast<uint32_t*>(&l);
-}
-// The same where no value is infinite: any weight, rounded, and the rest.
-__device__ __forceinline__ void two_rounded(float p0, float p1, uint32_t& hi, uint32_t& lo) {
-  __half2 h = __floats2half2_rn(p0, p1);
-  hi = *reinterpret_cast<uint32_t*>(&h);
-  const float2 c = __half22float2(h);
-  __half2 l = __floats2half2_rn(p0 - c.x, p1 - c.y);
-  lo = *reinterpret_cast<uint32_t*>(&l);
-}
-
-template <class T>
-__device__ __forceinline__ uint32_t pack2(float a, float b);
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) { return ako::pack_bf16x2(a, b); }
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
-  __half2 v = __floats2half2_rn(a, b);
-  return *reinterpret_cast<uint32_t*>(&v);
-}
-
-template <class T, int D>
-__device__ __forceinline__ void empty_head(const Params& p, int64_t row_head) {   // one thread
-  uint4* op = reinterpret_cast<uint4*>((T*)p.o + row_head * D);
-  for (int i = 0; i < D / 8; ++i) op[i] = make_uint4(0u, 0u, 0u, 0u);
-  p.lse[row_head] = -INFINITY;
-}
-
-// Where the tiles under way are: in registers, one of K and one of V, or (e4m3, which takes so long to work on that more
-// of them are needed, and 256 features, which are too many registers) in shared memory, some per warp.
-__host__ __device__ constexpr bool ringed(int64_t d, bool fp8) { return fp8 || d == 256; }
-__host__ __device__ constexpr int ctas_per_sm(int64_t, bool) { return 3; }
-__host__ __device__ constexpr int depth(int64_t d, bool fp8) { return !ringed(d, fp8) ? 1 : d * (fp8 ? 1 : 2) <= 64 ? 6 : d * (fp8 ? 1 : 2) <= 128 ? 4 : d * (fp8 ? 1 : 2) <= 256 ? 2 : 1; }
-// Bytes of shared memory of a warp: K and V of its tiles, the scales of a lane's two tokens.
-__host__ __device__ constexpr int ring_bytes(int64_t d, bool fp8) {
-  return ringed(d, fp8) ? depth(d, fp8) * (int)(2 * TILE * d * (fp8 ? 1 : 2) + (fp8 ? 512 : 0)) : 0;
-}
-// What a warp leaves for the others of its CTA: (m, l) of 8 heads, then O.
-__host__ __device__ constexpr int part_bytes(int64_t d) { return (8 * (int)d + 16) * 4; }
-
-template <class T, int D, bool FP8, bool ALIGNED>
-__global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_kernel(const Params p) {
-  constexpr int EB = FP8 ? 1 : 2;                  // bytes of a cache element
-  constexpr int NJ = D * EB / 64;                  // pieces per lane and token
-  constexpr int KS = D / 16;                       // steps of 16 features
-  constexpr bool RINGED = ringed(D, FP8);
-  constexpr int DEPTH = depth(D, FP8), RING = ring_bytes(D, FP8), HALF = 2 * NJ * 512;   // HALF: K, or V, of a tile
-  constexpr int PART = RINGED ? RING : part_bytes(D);
-  using TM = typename std::conditional<FP8, __half, T>::type;   // operand type
-  constexpr float LIFT = std::is_same<TM, __half>::value ? 15.f : 0.f;
-  __shared__ int s_scan[6];
-  extern __shared__ __align__(16) unsigned char s_ring[];   // [warp]: tiles, the scales of each; then its part
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, t = lane & 3;
-  ako::pdl_trigger();
-  // per_cta neighbouring (KV head, block) pairs of the same tokens; along warps for each, every along-th tile
-  const int share = blockIdx.x / p.unit_ctas, unit = (blockIdx.x % p.unit_ctas) * p.per_cta + warp % p.per_cta;
-  const int along = WARPS / p.per_cta, my = warp / p.per_cta;
-  const int kvh = unit / p.head_blocks, h0 = (unit % p.head_blocks) * 8;      // first head of the block in its group
-  const int heads = min(8, p.group - h0), head0 = kvh * p.group + h0;
-  const bool by_share = p.batch > p.shares;
-  const bool keeper = unit == 0 && threadIdx.x == 0;
-  const bool first_cta = blockIdx.x % p.unit_ctas == 0;
-  const ako::Share sh0 = ako::find_share(p.batch, share, p.shares, s_scan, [&](int r) { return span_of(p, r).tiles(); },
-                                         [&](int r) {
-                                           if (!first_cta) return;
-                                           for (int h = 0; h < p.q_heads; ++h) empty_head<T, D>(p, (int64_t)r * p.q_heads + h);
-                                           if (!by_share) p.cut[r] = cut_entry(r, 0, 0);
-                                         });
-  int2 cut = cut_entry(0, 0, 0);
-  int left = sh0.left, b = sh0.row, skip = sh0.skip;
-
-  const uint32_t ring = ako::smem_u32(s_ring) + warp * RING + lane * 16;
-  const uint4 *kbase[ALIGNED ? 2 : 1], *vbase[ALIGNED ? 2 : 1];       // ALIGNED: of tokens g and g + 8 of a tile
-  const float *kscale[ALIGNED ? 2 : 1], *vscales[ALIGNED ? 2 : 1];
-#pragma unroll
-  for (int i = 0; i < (ALIGNED ? 2 : 1); ++i) {
-    const uint32_t row = ALIGNED ? 8 * i + g : 0;
-    kbase[i] = p.k.data + (uint64_t)kvh * p.k.head + t + row * p.k.slot;
-    vbase[i] = p.v.data + (uint64_t)kvh * p.v.head + t + row * p.v.slot;
-    kscale[i] = p.k.scale + kvh * p.k.scale_head + row * p.k.scale_slot;
-    vscales[i] = p.v.scale + kvh * p.v.scale_head + row * p.v.scale_slot;
-  }
-  while (left > 0) {
-    const Span sp = span_of(p, b);
-    const int tiles = sp.tiles(), tile0 = sp.first_tile();
-    const int te = min(tiles, skip + left);
-    if (te <= skip) {                               // an empty sequence
-      ++b;
-      skip = 0;
-      continue;
-    }
-    left -= te - skip;
-    const int32_t* pages = p.table + (int64_t)b * p.max_pages;
-
-    // Where this lane's two tokens of a tile are. ALIGNED: pages are whole tiles, so that one page id and one slot
-    // do for all 16 (what follows the last token of a page is still the page's). Otherwise past the end: the last
-    // token. Tokens of a page that does not exist, and those past the end, are masked below.
-    constexpr int IDS = ALIGNED ? 1 : 2;
-    int id[IDS] = {}, slot[IDS] = {};
-    auto fetch_ids = [&](int tile) {
-#pragma unroll
-      for (int i = 0; i < IDS; ++i) {
-        const int tok = ALIGNED ? (tile0 + tile) * TILE : min((tile0 + tile) * TILE + 8 * i + g, sp.hi - 1);
-        const int page = p.page_shift >= 0 ? tok >> p.page_shift : (int)((unsigned)tok / (unsigned)p.page_size);
-        slot[i] = tok - page * p.page_size;
-        id[i] = __ldg(pages + page);
-      }
-    };
-    uint64_t voff[IDS], vscale[IDS];
-    uint32_t seen = 0;                              // two bits for each tile under way, the oldest on top
-    // Copies under way: K and V of a tile are a group each, in the order in which they are needed. A lane copies what
-    // it will read itself, so waiting for its own copies is all it takes.
-    uint4 kc[RINGED ? 1 : 2][RINGED ? 1 : NJ], vc[RINGED ? 1 : 2][RINGED ? 1 : NJ];
-    auto request_k = [&](int tile, uint32_t to) {
-      seen <<= 2;
-      if (tile < te) {
-        uint64_t off[IDS], ko[IDS];
-        bool real[IDS];
-#pragma unroll
-        for (int i = 0; i < IDS; ++i) {
-          real[i] = (unsigned)id[i] < (unsigned)p.num_pages;
-          const uint32_t page = real[i] ? id[i] : 0, sl = slot[i];
-          off[i] = (uint64_t)page * p.k.page + sl * p.k.slot;
-          voff[i] = p.same_strides ? off[i] : (uint64_t)page * p.v.page + sl * p.v.slot;
-          if (FP8) {
-            ko[i] = (uint64_t)page * p.k.scale_page + sl * p.k.scale_slot;
-            vscale[i] = p.same_strides ? ko[i] : (uint64_t)page * p.v.scale_page + sl * p.v.scale_slot;
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int tok = (tile0 + tile) * TILE + 8 * i + g;
-          seen |= (uint32_t)(real[ALIGNED ? 0 : i] && tok >= sp.lo && tok < sp.hi) << i;
-          const uint4* from = kbase[ALIGNED ? i : 0] + off[ALIGNED ? 0 : i];
-#pragma unroll
-          for (int j = 0; j < NJ; ++j) {
-            if (RINGED) ako::cp_async16(to + (i * NJ + j) * 512, from + 4 * j);
-            else kc[i][j] = ld16(from + 4 * j);
-          }
-          if (FP8) cp_async4(to + 2 * HALF + 4 * i, kscale[ALIGNED ? i : 0] + ko[ALIGNED ? 0 : i]);
-        }
-      }
-      if (RINGED) ako::cp_async_commit();
-    };
-    auto request_v = [&](int tile, uint32_t to) {
-      if (tile < te) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint4* from = vbase[ALIGNED ? i : 0] + voff[ALIGNED ? 0 : i];
-#pragma unroll
-          for (int j = 0; j < NJ; ++j) {
-            if (RINGED) ako::cp_async16(to + HALF + (i * NJ + j) * 512, from + 4 * j);
-            else vc[i][j] = ld16(from + 4 * j);
-          }
-          if (FP8) cp_async4(to + 2 * HALF + 8 + 4 * i, vscales[ALIGNED ? i : 0] + vscale[ALIGNED ? 0 : i]);
-        }
-      }
-      if (RINGED) ako::cp_async_commit();
-    };
-
-    // q of the block's heads as B fragments (n = head g), in the order of the K pieces
-    uint32_t qb[KS][2];
-#pragma unroll
-    for (int i = 0; i < KS; ++i) qb[i][0] = qb[i][1] = 0u;
-    if (g < heads) {
-      const unsigned char* qp = (const unsigned char*)p.q + ((int64_t)b * p.q_heads + head0 + g) * D * 2;
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        if (FP8) {                                  // 16 features, a word of K has four
-          const uint4 x = __ldg(reinterpret_cast<const uint4*>(qp + (64 * j + 16 * t) * 2));
-          const uint4 y = __ldg(reinterpret_cast<const uint4*>(qp + (64 * j + 16 * t + 8) * 2));
-          const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            qb[4 * j + i][0] = w[2 * i];
-            qb[4 * j + i][1] = w[2 * i + 1];
-          }
-        } else {
-          const uint4 x = __ldg(reinterpret_cast<const uint4*>(qp + (32 * j + 8 * t) * 2));
-          qb[2 * j][0] = x.x;
-          qb[2 * j][1] = x.y;
-          qb[2 * j + 1][0] = x.z;
-          qb[2 * j + 1][1] = x.w;
-        }
-      }
-    }
-    float qs0 = p.scale_log2, qs1 = p.scale_log2;   // of heads 2t and 2t + 1
-    if (FP8 && std::is_same<T, __nv_bfloat16>::value) {
-      // bf16 to fp16: times the power of two that brings the head's largest element to [1, 2). What falls below
-      // the fp16 range is off by 2^-25 of that.
-      float top = 0.f;
-#pragma unroll
-      for (int i = 0; i < KS; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) top = fmaxf(top, fmaxf(fabsf(ako::bf16_lo(qb[i][j])), fabsf(ako::bf16_hi(qb[i][j]))));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int e = exponent(top);
-      const float down = power_of_two(-e), back = power_of_two(e);
-#pragma unroll
-      for (int i = 0; i < KS; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) qb[i][j] = pack2<__half>(ako::bf16_lo(qb[i][j]) * down, ako::bf16_hi(qb[i][j]) * down);
-      qs0 *= __shfl_sync(0xffffffffu, back, 8 * t);
-      qs1 *= __shfl_sync(0xffffffffu, back, 8 * t + 4);
-    }
-    // e4m3: the weights of P times their scales, over 2^unit > all scales met so far, are what goes into the product
-    int unit_v = -121;
-    float over = 0.f, under = 0.f;                  // 2^unit, 2^-unit
-    // acc[i]: rows g and g + 8 of O^T step i, heads 2t and 2t + 1
-    float acc[KS][4];
-#pragma unroll
-    for (int i = 0; i < KS; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
-    // The maxima start at the lowest finite value, so that a score of -inf weighs 0 whatever else there is.
-    float m0 = -FLT_MAX, m1 = -FLT_MAX, l0 = 0.f, l1 = 0.f;
-
-    // slots of the ring: this one's address, each 2 HALF (+ 512) bytes
-    constexpr uint32_t SLOT = RING / DEPTH;
-    uint32_t at_slot = ring;
-    int ids[DEPTH][IDS], slots[DEPTH][IDS];
-#pragma unroll
-    for (int d = 0; d < DEPTH; ++d) {
-      if (skip + my + d * along < te) fetch_ids(skip + my + d * along);
-#pragma unroll
-      for (int i = 0; i < IDS; ++i) ids[d][i] = id[i], slots[d][i] = slot[i];
-    }
-#pragma unroll
-    for (int d = 0; d < DEPTH; ++d) {
-#pragma unroll
-      for (int i = 0; i < IDS; ++i) id[i] = ids[d][i], slot[i] = slots[d][i];
-      request_k(skip + my + d * along, ring + d * SLOT);
-      request_v(skip + my + d * along, ring + d * SLOT);
-    }
-    if (skip + my + DEPTH * along < te) fetch_ids(skip + my + DEPTH * along);
-    for (int tile = skip + my; tile < te; tile += along) {
-      if (RINGED) ako::cp_async_wait<2 * DEPTH - 1>();
-      float s[2][4] = {};                            // two chains of products, joined below
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const uint4 x = RINGED ? lds16(at_slot + j * 512) : kc[0][RINGED ? 0 : j], y = RINGED ? lds16(at_slot + (NJ + j) * 512) : kc[RINGED ? 0 : 1][RINGED ? 0 : j];
-        if (FP8) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t a[4];
-            widen(word(x, i), a[0], a[2]);
-            widen(word(y, i), a[1], a[3]);
-            mma<TM>(s[i & 1], a, qb[4 * j + i][0], qb[4 * j + i][1]);
-          }
-        } else {
-          const uint32_t a0[4] = {x.x, y.x, x.y, y.y}, a1[4] = {x.z, y.z, x.w, y.w};
-          mma<TM>(s[0], a0, qb[2 * j][0], qb[2 * j][1]);
-          mma<TM>(s[1], a1, qb[2 * j + 1][0], qb[2 * j + 1][1]);
-        }
-      }
-      float ks[2] = {1.f, 1.f};
-      if (FP8) lds_pair(at_slot + 2 * HALF, ks[0], ks[1]);
-      const bool now[2] = {(seen >> (2 * DEPTH - 2) & 1) != 0, (seen >> (2 * DEPTH - 1) & 1) != 0};
-      request_k(tile + DEPTH * along, at_slot);
-      // a lane's tokens, heads 2t and 2t + 1
-      float e[2][2];
-      float n0 = -INFINITY, n1 = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float x0 = s[0][2 * i] + s[1][2 * i], x1 = s[0][2 * i + 1] + s[1][2 * i + 1];
-        e[i][0] = now[i] ? x0 * (FP8 ? qs0 * ks[i] : qs0) : -INFINITY;
-        e[i][1] = now[i] ? x1 * (FP8 ? qs1 * ks[i] : qs1) : -INFINITY;
-        n0 = fmaxf(n0, e[i][0]);
-        n1 = fmaxf(n1, e[i][1]);
-      }
-#pragma unroll
-      for (int o = 4; o <= 16; o <<= 1) {
-        n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, o));
-        n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, o));
-      }
-      if (__any_sync(0xffffffffu, n0 > m0 || n1 > m1)) {
-        n0 = fmaxf(n0, m0);
-        n1 = fmaxf(n1, m1);
-        const float f0 = ako::fast_exp2(m0 - n0), f1 = ako::fast_exp2(m1 - n1);
-        m0 = n0;
-        m1 = n1;
-        l0 *= f0;
-        l1 *= f1;
-#pragma unroll
-        for (int i = 0; i < KS; ++i) {
-          acc[i][0] *= f0; acc[i][1] *= f1; acc[i][2] *= f0; acc[i][3] *= f1;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        e[i][0] = ako::fast_exp2(e[i][0] - m0 + LIFT);
-        e[i][1] = ako::fast_exp2(e[i][1] - m1 + LIFT);
-        l0 += e[i][0];
-        l1 += e[i][1];
-      }
-      if (RINGED) ako::cp_async_wait<2 * DEPTH - 1>();
-      if (!(now[0] && now[1])) {   // weight 0, but what was read in its place may hold anything
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < NJ; ++j)
-            if (!now[i]) {
-              if (RINGED) sts16(at_slot + HALF + (i * NJ + j) * 512, make_uint4(0u, 0u, 0u, 0u));
-              else vc[RINGED ? 0 : i][RINGED ? 0 : j] = make_uint4(0u, 0u, 0u, 0u);
-            }
-      }
-      if (FP8) {
-        float vs[2];
-        lds_pair(at_slot + 2 * HALF + 8, vs[0], vs[1]);
-        vs[0] = now[0] ? vs[0] : 0.f;
-        vs[1] = now[1] ? vs[1] : 0.f;
-        float top = fmaxf(fabsf(vs[0]), fabsf(vs[1]));
-        if (__any_sync(0xffffffffu, top >= over)) {
-#pragma unroll
-          for (int o = 4; o <= 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          const int u = max(unit_v, exponent(top) + 1);
-          if (u != unit_v) {
-            const float f = unit_v == -121 ? 0.f : power_of_two(max(unit_v - u, -126));
-#pragma unroll
-            for (int i = 0; i < KS; ++i)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) acc[i][j] *= f;
-            unit_v = u;
-            over = power_of_two(u);
-            under = power_of_two(-u);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float f = vs[i] * under;
-          e[i][0] *= f;
-          e[i][1] *= f;
-        }
-      }
-      uint32_t bh[2], bl[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (FP8) two_rounded(e[i][0], e[i][1], bh[i], bl[i]);
-        else two_pieces<TM>(e[i][0], e[i][1], bh[i], bl[i]);
-        bh[i] = ako::movmatrix_trans(bh[i]);
-        bl[i] = ako::movmatrix_trans(bl[i]);
-      }
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const uint4 x = RINGED ? lds16(at_slot + HALF + j * 512) : vc[0][RINGED ? 0 : j], y = RINGED ? lds16(at_slot + HALF + (NJ + j) * 512) : vc[RINGED ? 0 : 1][RINGED ? 0 : j];
-#pragma unroll
-        for (int i = 0; i < (FP8 ? 4 : 2); ++i) {
-          uint32_t x0, x1, y0, y1;
-          if (FP8) {
-            widen(word(x, i), x0, x1);
-            widen(word(y, i), y0, y1);
-          } else {
-            x0 = word(x, 2 * i), x1 = word(x, 2 * i + 1), y0 = word(y, 2 * i), y1 = word(y, 2 * i + 1);
-          }
-          const uint32_t a[4] = {ako::movmatrix_trans(x0), ako::movmatrix_trans(x1), ako::movmatrix_trans(y0), ako::movmatrix_trans(y1)};
-          float(&d)[4] = acc[(FP8 ? 4 : 2) * j + i];
-          mma<TM>(d, a, bl[0], bl[1]);
-          mma<TM>(d, a, bh[0], bh[1]);
-        }
-      }
-      request_v(tile + DEPTH * along, at_slot);
-      if (tile + (DEPTH + 1) * along < te) fetch_ids(tile + (DEPTH + 1) * along);
-      if (RINGED) {
-        at_slot += SLOT;
-        if (at_slot == ring + RING) at_slot = ring;
-      }
-    }
-#pragma unroll
-    for (int o = 4; o <= 16; o <<= 1) {
-      l0 += __shfl_xor_sync(0xffffffffu, l0, o);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, o);
-    }
-
-    if (FP8) {
-#pragma unroll
-      for (int i = 0; i < KS; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] *= over;
-    }
-    const bool whole = te - skip == tiles;
-    const int64_t at = by_share ? 2 * (int64_t)share + (skip == 0) : (int64_t)b + share;
-    if (skip == 0) {
-      cut = cut_entry(b, share, whole ? 1 : 1 + (tiles - te + sh0.per - 1) / sh0.per);
-      if (!by_share && keeper) p.cut[b] = cut;
-    }
-    // Lanes g = 2 x and 2 x + 1 hold the even and the odd of eight neighbouring features (16 bits) or of four and the next
-    // four (e4m3): swap, so that the even lane has the first four and the odd one the last four.
-    const bool odd = g & 1;
-    auto each_four = [&](auto&& put) {             // put(head of the block, feature, four values)
-#pragma unroll
-      for (int hh = 0; hh < 2; ++hh)
-#pragma unroll
-        for (int i = 0; i < KS; i += 2) {
-          const float a = acc[i][hh], c = acc[i][2 + hh], e = acc[i + 1][hh], f = acc[i + 1][2 + hh];
-          const float r0 = __shfl_xor_sync(0xffffffffu, odd ? a : e, 4), r1 = __shfl_xor_sync(0xffffffffu, odd ? c : f, 4);
-          const int col = FP8 ? 64 * (i / 4) + 16 * (g >> 1) + 4 * (i % 4) : 32 * (i / 2) + 8 * (g >> 1);
-          put(2 * t + hh, col + 4 * (g & 1), odd ? make_float4(r0, e, r1, f) : make_float4(a, r0, c, r1));
-        }
-    };
-    auto finish = [&](int h, int col, float4 x, float inv) {
-      if (h >= heads) return;
-      const int64_t head = head0 + h;
-      if (whole)
-        *reinterpret_cast<uint2*>((T*)p.o + ((int64_t)b * p.q_heads + head) * D + col) =
-            make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
-      else
-        *reinterpret_cast<float4*>(p.part_acc + (at * p.q_heads + head) * D + col) = x;
-    };
-    auto finish_ml = [&](int h, float m, float l) {
-      if (h >= heads) return;
-      const int64_t head = head0 + h;
-      if (whole) p.lse[(int64_t)b * p.q_heads + head] = l == 0.f ? -INFINITY : (m - LIFT) + log2f(l);
-      else *reinterpret_cast<float2*>(p.part_ml + (at * p.q_heads + head) * 2) = make_float2(m - LIFT, l);
-    };
-    if (along == 1) {
-      const float i0 = l0 == 0.f ? 0.f : 1.f / l0, i1 = l1 == 0.f ? 0.f : 1.f / l1;
-      each_four([&](int h, int col, float4 x) { finish(h, col, x, h & 1 ? i1 : i0); });
-      if (g == 0) {
-        finish_ml(2 * t, m0, l0);
-        finish_ml(2 * t + 1, m1, l1);
-      }
-    } else {
-      // the warps of a pair put theirs together, in order
-      auto part = [&](int w) { return reinterpret_cast<float*>(s_ring + w * PART); };
-      float* mine = part(warp);
-      __syncwarp();                                // every lane is through with the tiles
-      if (g == 0) {
-        mine[2 * t] = m0, mine[2 * t + 1] = m1;
-        mine[8 + 2 * t] = l0, mine[8 + 2 * t + 1] = l1;
-      }
-      each_four([&](int h, int col, float4 x) { *reinterpret_cast<float4*>(mine + 16 + h * D + col) = x; });
-      __syncthreads();
-      // this warp: heads my, my + along, ... of its pair
-      for (int h = my; h < heads; h += along) {
-        float M = -FLT_MAX, L = 0.f;
-        for (int i = 0; i < along; ++i) M = fmaxf(M, part(i * p.per_cta + warp % p.per_cta)[h]);
-        for (int i = 0; i < along; ++i) {
-          const float* x = part(i * p.per_cta + warp % p.per_cta);
-          L = fmaf(x[8 + h], exp2f(x[h] - M), L);
-        }
-        const float inv = L == 0.f ? 0.f : 1.f / L;
-        for (int col = 4 * lane; col < D; col += 128) {
-          float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int i = 0; i < along; ++i) {
-            const float* x = part(i * p.per_cta + warp % p.per_cta);
-            const float f = exp2f(x[h] - M);
-            const float4 y = *reinterpret_cast<const float4*>(x + 16 + h * D + col);
-            o = make_float4(fmaf(y.x, f, o.x), fmaf(y.y, f, o.y), fmaf(y.z, f, o.z), fmaf(y.w, f, o.w));
-          }
-          finish(h, col, o, inv);
-        }
-        if (lane == 0) finish_ml(h, M, L);
-      }
-      __syncthreads();                             // before the next segment's
-    }
-    ++b;
-    skip = 0;
-  }
-  if (by_share && keeper) p.cut[share] = cut;
-}
-
-// Merge. Few partials of a sequence: a warp per (sequence, head), lanes hold columns.
-constexpr int MERGE_MAX = 1024;                     // shares of a call never exceed this
-struct Cut {
-  int64_t row, slot0;
-  int n;
-  bool by_share;
-  __device__ __forceinline__ Cut(const Params& p, int64_t entry) {
-    const int2 c = p.cut[entry];
-    by_share = p.batch > p.shares;
-    row = c.x;
-    n = (unsigned)c.y >> 16;
-    slot0 = by_share ? 2 * (int64_t)(c.y & 0xffff) : row + (c.y & 0xffff);
-  }
-  __device__ __forceinline__ int64_t slot(int i) const { return slot0 + (by_share ? 2 * i + (i == 0) : i); }
-};
-template <class T, int D>
-__global__ void __launch_bounds__(128) paged_merge_few_kernel(const Params p) {
-  constexpr int C = D / 32;                         // columns per lane
-  const int lane = threadIdx.x & 31;
-  const int64_t job = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  ako::pdl_wait();
-  if (job >= (int64_t)min(p.batch, p.shares) * p.q_heads) return;
-  const int head = (int)(job % p.q_heads);
-  const Cut cut(p, job / p.q_heads);
-  if (cut.n <= 1) return;
-  float M = -FLT_MAX, L = 0.f, acc[C];
-#pragma unroll
-  for (int c = 0; c < C; ++c) acc[c] = 0.f;
-  for (int i0 = 0; i0 < cut.n; i0 += 32) {          // 32 partials at once, with their own maximum
-    float2 x = make_float2(-FLT_MAX, 0.f);
-    if (i0 + lane < cut.n) x = *reinterpret_cast<const float2*>(p.part_ml + (cut.slot(i0 + lane) * p.q_heads + head) * 2);
-    float top = fmaxf(M, x.x);
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float back = exp2f(M - top), f = exp2f(x.x - top);
-    M = top;
-    L = fmaf(L, back, x.y * f);
-#pragma unroll
-    for (int c = 0; c < C; ++c) acc[c] *= back;
-    const int k1 = min(32, cut.n - i0);
-#pragma unroll 4
-    for (int k = 0; k < k1; ++k) {
-      const float w = __shfl_sync(0xffffffffu, f, k);
-      const float* from = p.part_acc + (cut.slot(i0 + k) * p.q_heads + head) * D + lane * C;
-      float y[C];
-      if (C == 2) *reinterpret_cast<float2*>(y) = *reinterpret_cast<const float2*>(from);
-      else
-#pragma unroll
-        for (int c = 0; c < C; c += 4) *reinterpret_cast<float4*>(y + c) = *reinterpret_cast<const float4*>(from + c);
-#pragma unroll
-      for (int c = 0; c < C; ++c) acc[c] = fmaf(y[c], w, acc[c]);
-    }
-  }
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  const int64_t oi = cut.row * p.q_heads + head;
-  uint32_t* op = reinterpret_cast<uint32_t*>((T*)p.o + oi * D + lane * C);
-#pragma unroll
-  for (int c = 0; c < C; c += 2) op[c / 2] = pack2<T>(acc[c] * inv, acc[c + 1] * inv);
-  if (lane == 0) p.lse[oi] = L == 0.f ? -INFINITY : M + log2f(L);
-}
-// Many: a CTA per (sequence, head, 64 columns), a thread per partial for the weights, then 16 warps for every 16th one.
-constexpr int MERGE_WARPS = 16;
-template <class T, int D>
-__global__ void __launch_bounds__(MERGE_WARPS * 32) paged_merge_many_kernel(const Params p) {
-  constexpr int PER = MERGE_MAX / (MERGE_WARPS * 32);
-  __shared__ float s_w[MERGE_MAX], s_red[2][MERGE_WARPS];
-  __shared__ float2 s_acc[MERGE_WARPS][32];
-  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  const int block = blockIdx.x % (D / 64);
-  const int64_t job = blockIdx.x / (D / 64);
-  ako::pdl_wait();
-  const int head = (int)(job % p.q_heads);
-  const Cut cut(p, job / p.q_heads);
-  if (cut.n <= 1) return;
-  float2 x[PER];
-  float M = -FLT_MAX, L = 0.f;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int k = i * MERGE_WARPS * 32 + tid;
-    x[i] = make_float2(-FLT_MAX, 0.f);
-    if (k < cut.n) x[i] = *reinterpret_cast<const float2*>(p.part_ml + (cut.slot(k) * p.q_heads + head) * 2);
-    M = fmaxf(M, x[i].x);
-  }
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  if (lane == 0) s_red[0][w] = M;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < MERGE_WARPS; ++i) M = fmaxf(M, s_red[0][i]);
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const float f = exp2f(x[i].x - M);
-    s_w[i * MERGE_WARPS * 32 + tid] = f;
-    L = fmaf(x[i].y, f, L);
-  }
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-  if (lane == 0) s_red[1][w] = L;
-  __syncthreads();
-  float2 acc = make_float2(0.f, 0.f);
-#pragma unroll 8
-  for (int i = w; i < cut.n; i += MERGE_WARPS) {
-    const float f = s_w[i];
-    const float2 y = *reinterpret_cast<const float2*>(p.part_acc + (cut.slot(i) * p.q_heads + head) * D + block * 64 + lane * 2);
-    acc.x = fmaf(y.x, f, acc.x);
-    acc.y = fmaf(y.y, f, acc.y);
-  }
-  s_acc[w][lane] = acc;
-  __syncthreads();
-  if (w != 0) return;
-  L = s_red[1][0];
-#pragma unroll
-  for (int i = 1; i < MERGE_WARPS; ++i) {
-    acc.x += s_acc[i][lane].x;
-    acc.y += s_acc[i][lane].y;
-    L += s_red[1][i];
-  }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  const int64_t oi = cut.row * p.q_heads + head;
-  *reinterpret_cast<uint32_t*>((T*)p.o + oi * D + block * 64 + lane * 2) = pack2<T>(acc.x * inv, acc.y * inv);
-  if (lane == 0 && block == 0) p.lse[oi] = L == 0.f ? -INFINITY : M + log2f(L);
-}
-
-struct Plan {
-  int head_blocks, per_cta, unit_ctas;
-  int shares;
-  size_t ml, acc, total;   // offsets in the workspace; the entries are first
-};
-Plan plan_for(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t max_pages, int64_t page_size, int64_t window,
-              bool fp8) {
-  Plan pl;
-  pl.head_blocks = (int)ako::cdiv(q_heads / kv_heads, (int64_t)8);
-  const int64_t units = kv_heads * pl.head_blocks;
-  pl.per_cta = units % 4 == 0 ? 4 : units % 2 == 0 ? 2 : 1;
-  pl.unit_ctas = (int)(units / pl.per_cta);
-  // All CTAs resident at once, and a tile at least for a warp. What the lengths are is known on the device only.
-  const int64_t resident = (int64_t)ako::sm_count() * ctas_per_sm(dim, fp8);
-  int64_t tokens = max_pages * page_size;
-  if (window > 0 && tokens > window + TILE) tokens = window + TILE;
-  const int64_t tiles = batch * ako::cdiv(tokens, (int64_t)TILE);
-  int64_t shares = std::min(resident / pl.unit_ctas, ako::cdiv(tiles, (int64_t)(WARPS / pl.per_cta)));
-  pl.shares = (int)std::max<int64_t>(1, std::min<int64_t>(shares, MERGE_MAX));
-  const int64_t entries = std::min<int64_t>(batch, pl.shares), slots = entries + pl.shares;
-  pl.ml = (entries * sizeof(int2) + 255) / 256 * 256;
-  pl.acc = pl.ml + ((size_t)slots * q_heads * 8 + 255) / 256 * 256;
-  pl.total = pl.acc + (size_t)slots * q_heads * dim * 4;
-  return pl;
-}
 bool sizes_ok(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t max_pages, int64_t page_size, int64_t window) {
   const int64_t most = 0x7fffffffLL;
   return batch >= 0 && batch < most && q_heads > 0 && kv_heads > 0 && q_heads <= (1 << 16) && q_heads % kv_heads == 0 && page_size >= 1 &&
          page_size < most && max_pages >= 0 && max_pages < most && window >= 0 && (dim == 64 || dim == 128 || dim == 256);
-}
-
-template <class T, int D, bool FP8, bool ALIGNED>
-int launch(const Params& p, const Plan& pl, cudaStream_t st) {
-  constexpr int most = WARPS * (ringed(D, FP8) ? ring_bytes(D, FP8) : part_bytes(D));
-  static_assert(!ringed(D, FP8) || ring_bytes(D, FP8) >= part_bytes(D), "a warp's part is put where its tiles were");
-  if (!ako::ensure_dynamic_smem<paged_decode_kernel<T, D, FP8, ALIGNED>>(most)) return AKO4X_ELAUNCH;
-  const int smem = ringed(D, FP8) || pl.per_cta < WARPS ? most : 0;
-  paged_decode_kernel<T, D, FP8, ALIGNED><<<(unsigned)(pl.shares * pl.unit_ctas), THREADS, smem, st>>>(p);
-  AKO_CHECK_LAUNCH();
-  if (pl.shares == 1) return AKO4X_OK;
-  const int64_t jobs = (int64_t)std::min(p.batch, p.shares) * p.q_heads;
-  const bool many = p.shares >= 8LL * p.batch;      // partials of a sequence
-  const cudaError_t e = many ? ako::launch_pdl(true, paged_merge_many_kernel<T, D>, dim3((unsigned)jobs * (D / 64)), dim3(MERGE_WARPS * 32), 0, st, p)
-                             : ako::launch_pdl(true, paged_merge_few_kernel<T, D>, dim3((unsigned)ako::cdiv(jobs, (int64_t)4)), dim3(128), 0, st, p);
-  return e == cudaSuccess ? AKO4X_OK : AKO4X_ELAUNCH;
-}
-template <class T, int D, bool FP8>
-int launch(const Params& p, const Plan& pl, cudaStream_t st) {
-  return p.page_size % TILE == 0 ? launch<T, D, FP8, true>(p, pl, st) : launch<T, D, FP8, false>(p, pl, st);
-}
-template <class T, bool FP8>
-int launch(const Params& p, const Plan& pl, int64_t dim, cudaStream_t st) {
-  if (dim == 64) return launch<T, 64, FP8>(p, pl, st);
-  if (dim == 128) return launch<T, 128, FP8>(p, pl, st);
-  return launch<T, 256, FP8>(p, pl, st);
 }
 
 // A stride in units of `unit` elements, if it fits.
@@ -830,8 +61,7 @@ extern "C" int ako4x_paged_decode(const void* q, const ako4x_kv_cache* k_cache, 
   Params p = {};
   if ((!set_cache(p.k, k_cache, fp8, kv_heads, page_size) || !set_cache(p.v, v_cache, fp8, kv_heads, page_size)) && num_pages > 0)
     return AKO4X_EINVAL;
-  p.same_strides = p.k.page == p.v.page && p.k.slot == p.v.slot &&
-                   (!fp8 || (p.k.scale_page == p.v.scale_page && p.k.scale_slot == p.v.scale_slot && p.k.scale_head == p.v.scale_head));
+  p.same_strides = p.k.page == p.v.page && p.k.slot == p.v.slot;
   const Plan pl = plan_for(batch, q_heads, kv_heads, dim, max_pages, page_size, window, fp8);
   if (!workspace || workspace_bytes < pl.total) return AKO4X_EWORKSPACE;
   if ((uintptr_t)workspace & 15) return AKO4X_EINVAL;
@@ -859,6 +89,5 @@ extern "C" int ako4x_paged_decode(const void* q, const ako4x_kv_cache* k_cache, 
   p.window = (int)std::min<int64_t>(window, 0x7fffffff);
   p.shares = pl.shares;
   cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == AKO4X_BF16) return fp8 ? launch<__nv_bfloat16, true>(p, pl, dim, st) : launch<__nv_bfloat16, false>(p, pl, dim, st);
-  return fp8 ? launch<__half, true>(p, pl, dim, st) : launch<__half, false>(p, pl, dim, st);
+  return dtype == AKO4X_BF16 ? run_bf16(p, pl, dim, fp8, st) : run_fp16(p, pl, dim, fp8, st);
 }
