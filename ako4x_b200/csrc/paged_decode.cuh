@@ -39,7 +39,7 @@
 namespace ako {
 namespace paged {
 
-constexpr int TILE = 16;
+constexpr int BLOCK = 16;   // tokens of a matrix product
 
 constexpr int WARPS = 4, THREADS = WARPS * 32;
 
@@ -72,14 +72,16 @@ struct Params {
 // share, for the sequence that starts in it and goes on (slot 2 share, the first one of a sequence 2 share + 1).
 __device__ __forceinline__ int2 cut_entry(int b, int first, int n) { return make_int2(b, first | n << 16); }
 
+template <int TILE>
 struct Span {          // visible tokens of a sequence
   int lo, hi;
   __device__ __forceinline__ int first_tile() const { return lo / TILE; }
   __device__ __forceinline__ int tiles() const { return hi > lo ? (hi + TILE - 1) / TILE - lo / TILE : 0; }
 };
-__device__ __forceinline__ Span span_of(const Params& p, int b) {
+template <int TILE>
+__device__ __forceinline__ Span<TILE> span_of(const Params& p, int b) {
   const int64_t most = min((int64_t)p.max_pages * p.page_size, (int64_t)0x7fffff00);   // tiles end in 32 bits
-  Span s;
+  Span<TILE> s;
   s.hi = p.num_pages > 0 ? (int)min((int64_t)max(0, p.lens[b]), most) : 0;
   s.lo = p.window > 0 ? max(0, s.hi - p.window) : 0;
   return s;
@@ -174,10 +176,13 @@ __device__ __forceinline__ void empty_head(const Params& p, int64_t row_head) { 
 // of them are needed, and 256 features, which are too many registers) in shared memory, some per warp.
 __host__ __device__ constexpr bool ringed(int64_t d, bool fp8) { return fp8 || d == 256; }
 __host__ __device__ constexpr int ctas_per_sm(int64_t, bool) { return 3; }
-__host__ __device__ constexpr int depth(int64_t d, bool fp8) { return !ringed(d, fp8) ? 1 : d * (fp8 ? 1 : 2) <= 64 ? 6 : d * (fp8 ? 1 : 2) <= 128 ? 4 : d * (fp8 ? 1 : 2) <= 256 ? 2 : 1; }
-// Bytes of shared memory of a warp: K and V of its tiles, and the scales of their tokens (a quad of lanes: K's two, V's two).
+// Blocks of a tile: two in e4m3 (64 and 128 features), whose work on a block is a long chain.
+__host__ __device__ constexpr int blocks(int64_t d, bool fp8) { return fp8 && d <= 128 ? 2 : 1; }
+__host__ __device__ constexpr int depth(int64_t d, bool fp8) { return fp8 ? (d == 64 ? 3 : 2) : 1; }
+// Bytes of shared memory of a warp: K and V of its tiles, and the scales of their tokens (a quad of lanes: K's two, V's
+// two, for each block).
 __host__ __device__ constexpr int ring_bytes(int64_t d, bool fp8) {
-  return ringed(d, fp8) ? depth(d, fp8) * (int)(2 * TILE * d * (fp8 ? 1 : 2) + (fp8 ? 128 : 0)) : 0;
+  return ringed(d, fp8) ? depth(d, fp8) * blocks(d, fp8) * (int)(2 * BLOCK * d * (fp8 ? 1 : 2) + (fp8 ? 128 : 0)) : 0;
 }
 // What a warp leaves for the others of its CTA: (m, l) of 8 heads, then O.
 __host__ __device__ constexpr int part_bytes(int64_t d) { return (8 * (int)d + 16) * 4; }
@@ -188,7 +193,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
   constexpr int NJ = D * EB / 64;                  // pieces per lane and token
   constexpr int KS = D / 16;                       // steps of 16 features
   constexpr bool RINGED = ringed(D, FP8);
-  constexpr int DEPTH = depth(D, FP8), RING = ring_bytes(D, FP8), HALF = 2 * NJ * 512;   // HALF: K, or V, of a tile
+  constexpr int TT = blocks(D, FP8), TILE = BLOCK * TT, R = 2 * TT;   // R: tokens of a lane in a tile
+  constexpr int DEPTH = depth(D, FP8), RING = ring_bytes(D, FP8), HALF = R * NJ * 512;   // HALF: K, or V, of a tile
   constexpr int PART = RINGED ? RING : part_bytes(D);
   using TM = typename std::conditional<FP8, __half, T>::type;   // operand type
   constexpr float LIFT = std::is_same<TM, __half>::value ? 15.f : 0.f;
@@ -205,7 +211,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
   const bool by_share = p.batch > p.shares;
   const bool keeper = unit == 0 && threadIdx.x == 0;
   const bool first_cta = blockIdx.x % p.unit_ctas == 0;
-  const ako::Share sh0 = ako::find_share(p.batch, share, p.shares, s_scan, [&](int r) { return span_of(p, r).tiles(); },
+  const ako::Share sh0 = ako::find_share(p.batch, share, p.shares, s_scan, [&](int r) { return span_of<TILE>(p, r).tiles(); },
                                          [&](int r) {
                                            if (!first_cta) return;
                                            for (int h = 0; h < p.q_heads; ++h) empty_head<T, D>(p, (int64_t)r * p.q_heads + h);
@@ -227,7 +233,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
   const uint32_t sc_page = sc.scale_page, sc_slot = sc.scale_slot;
   const float* sc_base = sc.scale + kvh * sc.scale_head + (ALIGNED ? (8 * (t & 1) + g) * sc_slot : 0);
   while (left > 0) {
-    const Span sp = span_of(p, b);
+    const Span<TILE> sp = span_of<TILE>(p, b);
     const int tiles = sp.tiles(), tile0 = sp.first_tile();
     const int te = min(tiles, skip + left);
     if (te <= skip) {                               // an empty sequence
@@ -238,27 +244,29 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
     left -= te - skip;
     const int32_t* pages = p.table + (int64_t)b * p.max_pages;
 
-    // Where this lane's two tokens of a tile are. ALIGNED: pages are whole tiles, so that one page id and one slot
-    // do for all 16 (what follows the last token of a page is still the page's). Otherwise past the end: the last
-    // token. Tokens of a page that does not exist, and those past the end, are masked below.
-    constexpr int IDS = ALIGNED ? 1 : 2;
+    // Where this lane's tokens of a tile are. ALIGNED: pages are whole blocks, so that one page id and one slot
+    // do for all 16 tokens (what follows the last token of a page is still the page's). Past the end: the last
+    // block, or token. Tokens of a page that does not exist, and those past the end, are masked below.
+    constexpr int IDS = ALIGNED ? TT : R;
     int id[IDS] = {}, slot[IDS] = {};
     auto fetch_ids = [&](int tile) {
 #pragma unroll
       for (int i = 0; i < IDS; ++i) {
-        const int tok = ALIGNED ? (tile0 + tile) * TILE : min((tile0 + tile) * TILE + 8 * i + g, sp.hi - 1);
+        const int tok = ALIGNED ? min((tile0 + tile) * TILE + BLOCK * i, (sp.hi - 1) / BLOCK * BLOCK)
+                                : min((tile0 + tile) * TILE + 8 * i + g, sp.hi - 1);
         const int page = p.page_shift >= 0 ? tok >> p.page_shift : (int)((unsigned)tok / (unsigned)p.page_size);
         slot[i] = tok - page * p.page_size;
         id[i] = __ldg(pages + page);
       }
     };
     uint64_t voff[IDS];
-    uint32_t seen = 0;                              // two bits for each tile under way, the oldest on top
+    uint32_t seen = 0;                              // R bits for each tile under way, the oldest on top
     // Copies under way: K and V of a tile are a group each, in the order in which they are needed. A lane copies what
     // it will read itself, so waiting for its own copies is all it takes.
-    uint4 kc[RINGED ? 1 : 2][RINGED ? 1 : NJ], vc[RINGED ? 1 : 2][RINGED ? 1 : NJ];
+    uint4 kc[RINGED ? 1 : R][RINGED ? 1 : NJ], vc[RINGED ? 1 : R][RINGED ? 1 : NJ];
+    float scn[TT];
     auto request_k = [&](int tile, uint32_t to) {
-      seen <<= 2;
+      seen <<= R;
       if (tile < te) {
         uint64_t off[IDS];
         bool real[IDS];
@@ -268,17 +276,21 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
           const uint32_t page = real[i] ? id[i] : 0, sl = slot[i];
           off[i] = (uint64_t)page * p.k.page + sl * p.k.slot;
           voff[i] = p.same_strides ? off[i] : (uint64_t)page * p.v.page + sl * p.v.slot;
-          if (FP8 && (ALIGNED || i == (t & 1))) cp_async4(to - lane * 12 + 2 * HALF, sc_base + ((uint64_t)page * sc_page + sl * sc_slot));
+          if (FP8 && (ALIGNED || (i & 1) == (t & 1))) {
+            const float* from = sc_base + ((uint64_t)page * sc_page + sl * sc_slot);
+            if (RINGED) cp_async4(to - lane * 12 + 2 * HALF + (ALIGNED ? i : i / 2) * 128, from);
+            else scn[ALIGNED ? i : i / 2] = __ldg(from);
+          }
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < R; ++i) {
           const int tok = (tile0 + tile) * TILE + 8 * i + g;
-          seen |= (uint32_t)(real[ALIGNED ? 0 : i] && tok >= sp.lo && tok < sp.hi) << i;
-          const uint4* from = kbase[ALIGNED ? i : 0] + off[ALIGNED ? 0 : i];
+          seen |= (uint32_t)(real[ALIGNED ? i / 2 : i] && tok >= sp.lo && tok < sp.hi) << i;
+          const uint4* from = kbase[ALIGNED ? i & 1 : 0] + off[ALIGNED ? i / 2 : i];
 #pragma unroll
           for (int j = 0; j < NJ; ++j) {
             if (RINGED) ako::cp_async16(to + (i * NJ + j) * 512, from + 4 * j);
-            else kc[i][j] = ld16(from + 4 * j);
+            else kc[RINGED ? 0 : i][RINGED ? 0 : j] = ld16(from + 4 * j);
           }
         }
       }
@@ -287,12 +299,12 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
     auto request_v = [&](int tile, uint32_t to) {
       if (tile < te) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint4* from = vbase[ALIGNED ? i : 0] + voff[ALIGNED ? 0 : i];
+        for (int i = 0; i < R; ++i) {
+          const uint4* from = vbase[ALIGNED ? i & 1 : 0] + voff[ALIGNED ? i / 2 : i];
 #pragma unroll
           for (int j = 0; j < NJ; ++j) {
             if (RINGED) ako::cp_async16(to + HALF + (i * NJ + j) * 512, from + 4 * j);
-            else vc[i][j] = ld16(from + 4 * j);
+            else vc[RINGED ? 0 : i][RINGED ? 0 : j] = ld16(from + 4 * j);
           }
         }
       }
@@ -379,40 +391,56 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
     if (skip + my + DEPTH * along < te) fetch_ids(skip + my + DEPTH * along);
     for (int tile = skip + my; tile < te; tile += along) {
       if (RINGED) ako::cp_async_wait<2 * DEPTH - 1>();
-      float s[2][4] = {};                            // two chains of products, joined below
+      float s[TT][2][4] = {};                        // two chains of products for a block, joined below
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const uint4 x = RINGED ? lds16(at_slot + j * 512) : kc[0][RINGED ? 0 : j], y = RINGED ? lds16(at_slot + (NJ + j) * 512) : kc[RINGED ? 0 : 1][RINGED ? 0 : j];
-        if (FP8) {
+      for (int j = 0; j < NJ; ++j)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t a[4];
-            widen(word(x, i), a[0], a[2]);
-            widen(word(y, i), a[1], a[3]);
-            mma<TM>(s[i & 1], a, qb[4 * j + i][0], qb[4 * j + i][1]);
+        for (int u = 0; u < TT; ++u) {
+          const uint4 x = RINGED ? lds16(at_slot + (2 * u * NJ + j) * 512) : kc[RINGED ? 0 : 2 * u][RINGED ? 0 : j];
+          const uint4 y = RINGED ? lds16(at_slot + ((2 * u + 1) * NJ + j) * 512) : kc[RINGED ? 0 : 2 * u + 1][RINGED ? 0 : j];
+          if (FP8) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t a[4];
+              widen(word(x, i), a[0], a[2]);
+              widen(word(y, i), a[1], a[3]);
+              mma<TM>(s[u][i & 1], a, qb[4 * j + i][0], qb[4 * j + i][1]);
+            }
+          } else {
+            const uint32_t a0[4] = {x.x, y.x, x.y, y.y}, a1[4] = {x.z, y.z, x.w, y.w};
+            mma<TM>(s[u][0], a0, qb[2 * j][0], qb[2 * j][1]);
+            mma<TM>(s[u][1], a1, qb[2 * j + 1][0], qb[2 * j + 1][1]);
           }
-        } else {
-          const uint32_t a0[4] = {x.x, y.x, x.y, y.y}, a1[4] = {x.z, y.z, x.w, y.w};
-          mma<TM>(s[0], a0, qb[2 * j][0], qb[2 * j][1]);
-          mma<TM>(s[1], a1, qb[2 * j + 1][0], qb[2 * j + 1][1]);
         }
-      }
-      float ks[2] = {1.f, 1.f}, vs[2];
+      float ks[R], vs[R];
       if (FP8) {
-        __syncwarp();                                // the quad's copies have arrived
-        const uint4 x = lds16(at_slot - lane * 16 + 2 * HALF + (lane & ~3) * 4);
-        ks[0] = __uint_as_float(x.x), ks[1] = __uint_as_float(x.y);
-        vs[0] = __uint_as_float(x.z), vs[1] = __uint_as_float(x.w);
-        __syncwarp();                                // and been read before the next ones
+        if (RINGED) __syncwarp();                    // the quad's copies have arrived
+#pragma unroll
+        for (int u = 0; u < TT; ++u) {
+          if (!RINGED) {
+            ks[2 * u] = __shfl_sync(0xffffffffu, scn[u], lane & ~3), ks[2 * u + 1] = __shfl_sync(0xffffffffu, scn[u], lane & ~3 | 1);
+            vs[2 * u] = __shfl_sync(0xffffffffu, scn[u], lane & ~3 | 2), vs[2 * u + 1] = __shfl_sync(0xffffffffu, scn[u], lane | 3);
+            continue;
+          }
+          const uint4 x = lds16(at_slot - lane * 16 + 2 * HALF + u * 128 + (lane & ~3) * 4);
+          ks[2 * u] = __uint_as_float(x.x), ks[2 * u + 1] = __uint_as_float(x.y);
+          vs[2 * u] = __uint_as_float(x.z), vs[2 * u + 1] = __uint_as_float(x.w);
+        }
+        if (RINGED) __syncwarp();                    // and been read before the next ones
       }
-      const bool now[2] = {(seen >> (2 * DEPTH - 2) & 1) != 0, (seen >> (2 * DEPTH - 1) & 1) != 0};
+      bool now[R], all = true;
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        now[i] = (seen >> (R * (DEPTH - 1) + i) & 1) != 0;
+        all &= now[i];
+      }
       request_k(tile + DEPTH * along, at_slot);
       // a lane's tokens, heads 2t and 2t + 1
-      float e[2][2];
+      float e[R][2];
       float n0 = -INFINITY, n1 = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float x0 = s[0][2 * i] + s[1][2 * i], x1 = s[0][2 * i + 1] + s[1][2 * i + 1];
+      for (int i = 0; i < R; ++i) {
+        const float x0 = s[i / 2][0][2 * (i & 1)] + s[i / 2][1][2 * (i & 1)], x1 = s[i / 2][0][2 * (i & 1) + 1] + s[i / 2][1][2 * (i & 1) + 1];
         e[i][0] = now[i] ? x0 * (FP8 ? qs0 * ks[i] : qs0) : -INFINITY;
         e[i][1] = now[i] ? x1 * (FP8 ? qs1 * ks[i] : qs1) : -INFINITY;
         n0 = fmaxf(n0, e[i][0]);
@@ -437,16 +465,16 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
         }
       }
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < R; ++i) {
         e[i][0] = ako::fast_exp2(e[i][0] - m0 + LIFT);
         e[i][1] = ako::fast_exp2(e[i][1] - m1 + LIFT);
         l0 += e[i][0];
         l1 += e[i][1];
       }
       if (RINGED) ako::cp_async_wait<2 * DEPTH - 1>();
-      if (!(now[0] && now[1])) {   // weight 0, but what was read in its place may hold anything
+      if (!all) {   // weight 0, but what was read in its place may hold anything
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < R; ++i)
 #pragma unroll
           for (int j = 0; j < NJ; ++j)
             if (!now[i]) {
@@ -455,9 +483,12 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
             }
       }
       if (FP8) {
-        vs[0] = now[0] ? vs[0] : 0.f;
-        vs[1] = now[1] ? vs[1] : 0.f;
-        float top = fmaxf(fabsf(vs[0]), fabsf(vs[1]));
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          vs[i] = now[i] ? vs[i] : 0.f;
+          top = fmaxf(top, fabsf(vs[i]));
+        }
         if (__any_sync(0xffffffffu, top >= over)) {
 #pragma unroll
           for (int o = 4; o <= 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -474,15 +505,15 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
           }
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < R; ++i) {
           const float f = vs[i] * under;
           e[i][0] *= f;
           e[i][1] *= f;
         }
       }
-      uint32_t bh[2], bl[2];
+      uint32_t bh[R], bl[R];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < R; ++i) {
         if (FP8) two_rounded(e[i][0], e[i][1], bh[i], bl[i]);
         else two_pieces<TM>(e[i][0], e[i][1], bh[i], bl[i]);
         if (FOLD) {
@@ -493,23 +524,26 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
         }
       }
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const uint4 x = RINGED ? lds16(at_slot + HALF + j * 512) : vc[0][RINGED ? 0 : j], y = RINGED ? lds16(at_slot + HALF + (NJ + j) * 512) : vc[RINGED ? 0 : 1][RINGED ? 0 : j];
+      for (int j = 0; j < NJ; ++j)
 #pragma unroll
-        for (int i = 0; i < (FP8 ? 4 : 2); ++i) {
-          uint32_t x0, x1, y0, y1;
-          if (FP8) {
-            widen(word(x, i), x0, x1);
-            widen(word(y, i), y0, y1);
-          } else {
-            x0 = word(x, 2 * i), x1 = word(x, 2 * i + 1), y0 = word(y, 2 * i), y1 = word(y, 2 * i + 1);
+        for (int u = 0; u < TT; ++u) {
+          const uint4 x = RINGED ? lds16(at_slot + HALF + (2 * u * NJ + j) * 512) : vc[RINGED ? 0 : 2 * u][RINGED ? 0 : j];
+          const uint4 y = RINGED ? lds16(at_slot + HALF + ((2 * u + 1) * NJ + j) * 512) : vc[RINGED ? 0 : 2 * u + 1][RINGED ? 0 : j];
+#pragma unroll
+          for (int i = 0; i < (FP8 ? 4 : 2); ++i) {
+            uint32_t x0, x1, y0, y1;
+            if (FP8) {
+              widen(word(x, i), x0, x1);
+              widen(word(y, i), y0, y1);
+            } else {
+              x0 = word(x, 2 * i), x1 = word(x, 2 * i + 1), y0 = word(y, 2 * i), y1 = word(y, 2 * i + 1);
+            }
+            const uint32_t a[4] = {ako::movmatrix_trans(x0), ako::movmatrix_trans(x1), ako::movmatrix_trans(y0), ako::movmatrix_trans(y1)};
+            float(&d)[4] = acc[(FP8 ? 4 : 2) * j + i];
+            if (!FOLD) mma<TM>(d, a, bl[2 * u], bl[2 * u + 1]);
+            mma<TM>(d, a, bh[2 * u], bh[2 * u + 1]);
           }
-          const uint32_t a[4] = {ako::movmatrix_trans(x0), ako::movmatrix_trans(x1), ako::movmatrix_trans(y0), ako::movmatrix_trans(y1)};
-          float(&d)[4] = acc[(FP8 ? 4 : 2) * j + i];
-          if (!FOLD) mma<TM>(d, a, bl[0], bl[1]);
-          mma<TM>(d, a, bh[0], bh[1]);
         }
-      }
       request_v(tile + DEPTH * along, at_slot);
       if (tile + (DEPTH + 1) * along < te) fetch_ids(tile + (DEPTH + 1) * along);
       if (RINGED) {
@@ -753,6 +787,7 @@ inline Plan plan_for(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t d
   pl.unit_ctas = (int)(units / pl.per_cta);
   // All CTAs resident at once, and a tile at least for a warp. What the lengths are is known on the device only.
   const int64_t resident = (int64_t)ako::sm_count() * ctas_per_sm(dim, fp8);
+  const int64_t TILE = BLOCK * blocks(dim, fp8);
   int64_t tokens = max_pages * page_size;
   if (window > 0 && tokens > window + TILE) tokens = window + TILE;
   const int64_t tiles = batch * ako::cdiv(tokens, (int64_t)TILE);
@@ -782,7 +817,7 @@ int launch(const Params& p, const Plan& pl, cudaStream_t st) {
 template <class T, int D, bool FP8>
 int launch(const Params& p, const Plan& pl, cudaStream_t st) {
   const bool fold = p.group <= 4;
-  if (p.page_size % TILE == 0) return fold ? launch<T, D, FP8, true, true>(p, pl, st) : launch<T, D, FP8, true, false>(p, pl, st);
+  if (p.page_size % BLOCK == 0) return fold ? launch<T, D, FP8, true, true>(p, pl, st) : launch<T, D, FP8, true, false>(p, pl, st);
   return fold ? launch<T, D, FP8, false, true>(p, pl, st) : launch<T, D, FP8, false, false>(p, pl, st);
 }
 template <class T, bool FP8>
