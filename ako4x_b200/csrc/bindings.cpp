@@ -806,35 +806,64 @@ PyObject* paged_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 // ---- pages of a cache ----
 
+// Whether what lies behind the first dimension is one piece of memory, in whatever order.
+bool one_piece(const Tensor& x) {
+  const IntArrayRef sizes = x.sizes(), strides = x.strides();
+  int64_t next = 1;
+  for (size_t left = sizes.size() - 1, d = left; d >= 1; --d) {   // the usual order
+    if (sizes[d] != 1 && strides[d] != next) break;
+    next *= sizes[d];
+    if (--left == 0) return true;
+  }
+  if (sizes.size() == 1) return true;
+  next = 1;
+  std::vector<bool> taken(sizes.size(), false);
+  for (size_t n = 1; n < sizes.size(); ++n) {                     // any order: the dimension with the next stride
+    size_t found = 0;
+    for (size_t d = 1; d < sizes.size() && !found; ++d)
+      if (!taken[d] && (sizes[d] == 1 || strides[d] == next)) found = d;
+    if (!found) return false;
+    taken[found] = true;
+    next *= sizes[found];
+  }
+  return true;
+}
 // The tensors that have pages along their first dimension.
 struct PagedTensors {
-  std::vector<Tensor> t;
+  PyObject* seq;
+  std::vector<const Tensor*> t;
   std::vector<void*> data;
   std::vector<int64_t> bytes, strides;
+  int64_t num_pages;
   PagedTensors(const char* op, PyObject* list, int64_t pages) {   // pages < 0: those of the first one
-    PyObject* seq = PySequence_Fast(list, "caches: a list of tensors expected");
+    seq = PySequence_Fast(list, "caches: a list of tensors expected");
     if (!seq) throw python_error();
     try {
-      for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(seq); ++i) t.push_back(tensor(PySequence_Fast_GET_ITEM(seq, i)));
+      const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq);
+      t.reserve(n);
+      data.reserve(n);
+      bytes.reserve(n);
+      strides.reserve(n);
+      for (Py_ssize_t i = 0; i < n; ++i) {
+        const Tensor& x = tensor(PySequence_Fast_GET_ITEM(seq, i));
+        t.push_back(&x);
+        if (x.dim() >= 1 && pages < 0) pages = x.size(0);
+        if (x.dim() < 1 || x.size(0) != pages) fail(std::string(op) + ": every cache must have the pages along its first dimension");
+        if (x.numel() == 0) continue;
+        const int64_t per = x.numel() / pages;
+        if (!(one_piece(x) && (pages == 1 || x.stride(0) >= per))) fail(std::string(op) + ": a page of a cache must be one piece of memory");
+        data.push_back(x.data_ptr());
+        bytes.push_back(per * (int64_t)x.element_size());
+        strides.push_back(pages == 1 ? bytes.back() : x.stride(0) * (int64_t)x.element_size());
+      }
     } catch (...) {
       Py_DECREF(seq);
       throw;
     }
-    Py_DECREF(seq);
-    for (const Tensor& x : t) {
-      if (x.dim() >= 1 && pages < 0) pages = x.size(0);
-      if (x.dim() < 1 || x.size(0) != pages) fail(std::string(op) + ": every cache must have the pages along its first dimension");
-      if (x.numel() == 0) continue;
-      const int64_t per = x.numel() / pages;
-      if (!(x.select(0, 0).is_non_overlapping_and_dense() && (pages == 1 || x.stride(0) >= per)))
-        fail(std::string(op) + ": a page of a cache must be one piece of memory");
-      data.push_back(x.data_ptr());
-      bytes.push_back(per * (int64_t)x.element_size());
-      strides.push_back(pages == 1 ? bytes.back() : x.stride(0) * (int64_t)x.element_size());
-    }
     num_pages = pages;
   }
-  int64_t num_pages;
+  PagedTensors(const PagedTensors&) = delete;
+  ~PagedTensors() { Py_DECREF(seq); }
   int64_t count() const { return (int64_t)data.size(); }
 };
 // The state, changed in place: block_table int32 [rows, max_pages], seq_lens int32 [rows], ref_counts int32 [pages].
@@ -854,11 +883,11 @@ int64_t page_size_of(const char* op, PyObject* o) {
 }
 OneDevice device_of(const char* op, std::initializer_list<const Tensor*> all, const PagedTensors* caches) {
   if (caches)
-    for (const Tensor& t : caches->t)
+    for (const Tensor* t : caches->t) {
+      need(t->is_cuda(), "ako4x_b200 operators take CUDA tensors only (there is no CPU path)");
       for (const Tensor* x : all)
-        if (t.is_cuda() && x->is_cuda() && t.device() != x->device()) fail(std::string(op) + ": tensors on different devices");
-  if (caches)
-    for (const Tensor& t : caches->t) need(t.is_cuda(), "ako4x_b200 operators take CUDA tensors only (there is no CPU path)");
+        if (x->is_cuda() && t->device() != x->device()) fail(std::string(op) + ": tensors on different devices");
+    }
   return OneDevice(op, all);
 }
 

@@ -89,7 +89,7 @@ __device__ __forceinline__ Span<TILE> span_of(const Params& p, int b) {
 
 __device__ __forceinline__ uint4 ld16(const uint4* p) {
   uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
   return r;
 }
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
@@ -203,6 +203,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   ako::pdl_trigger();
+  ako::pdl_wait();   // its launch is hidden behind the kernel before; no load here is of the read-only kind
   // per_cta neighbouring (KV head, block) pairs of the same tokens; along warps for each, every along-th tile
   const int share = blockIdx.x / p.unit_ctas, unit = (blockIdx.x % p.unit_ctas) * p.per_cta + warp % p.per_cta;
   const int along = WARPS / p.per_cta, my = warp / p.per_cta;
@@ -256,7 +257,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
                                 : min((tile0 + tile) * TILE + 8 * i + g, sp.hi - 1);
         const int page = p.page_shift >= 0 ? tok >> p.page_shift : (int)((unsigned)tok / (unsigned)p.page_size);
         slot[i] = tok - page * p.page_size;
-        id[i] = __ldg(pages + page);
+        id[i] = pages[page];
       }
     };
     uint64_t voff[IDS];
@@ -279,7 +280,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
           if (FP8 && (ALIGNED || (i & 1) == (t & 1))) {
             const float* from = sc_base + ((uint64_t)page * sc_page + sl * sc_slot);
             if (RINGED) cp_async4(to - lane * 12 + 2 * HALF + (ALIGNED ? i : i / 2) * 128, from);
-            else scn[ALIGNED ? i : i / 2] = __ldg(from);
+            else scn[ALIGNED ? i : i / 2] = *from;
           }
         }
 #pragma unroll
@@ -322,8 +323,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
         if (FP8) {                                  // 16 features, a word of K has four
-          const uint4 x = __ldg(reinterpret_cast<const uint4*>(qp + (64 * j + 16 * t) * 2));
-          const uint4 y = __ldg(reinterpret_cast<const uint4*>(qp + (64 * j + 16 * t + 8) * 2));
+          const uint4 x = *reinterpret_cast<const uint4*>(qp + (64 * j + 16 * t) * 2);
+          const uint4 y = *reinterpret_cast<const uint4*>(qp + (64 * j + 16 * t + 8) * 2);
           const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -331,7 +332,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
             qb[4 * j + i][1] = w[2 * i + 1];
           }
         } else {
-          const uint4 x = __ldg(reinterpret_cast<const uint4*>(qp + (32 * j + 8 * t) * 2));
+          const uint4 x = *reinterpret_cast<const uint4*>(qp + (32 * j + 8 * t) * 2);
           qb[2 * j][0] = x.x;
           qb[2 * j][1] = x.y;
           qb[2 * j + 1][0] = x.z;
@@ -668,6 +669,7 @@ __global__ void __launch_bounds__(128) paged_merge_few_kernel(const Params p) {
   constexpr int C = D / 32;                         // columns per lane
   const int lane = threadIdx.x & 31;
   const int64_t job = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  ako::pdl_trigger();
   ako::pdl_wait();
   if (job >= (int64_t)min(p.batch, p.shares) * p.q_heads) return;
   const int head = (int)(job % p.q_heads);
@@ -720,6 +722,7 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) paged_merge_many_kernel(cons
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int block = blockIdx.x % (D / 64);
   const int64_t job = blockIdx.x / (D / 64);
+  ako::pdl_trigger();
   ako::pdl_wait();
   const int head = (int)(job % p.q_heads);
   const Cut cut(p, job / p.q_heads);
@@ -805,8 +808,9 @@ int launch(const Params& p, const Plan& pl, cudaStream_t st) {
   static_assert(!ringed(D, FP8) || ring_bytes(D, FP8) >= part_bytes(D), "a warp's part is put where its tiles were");
   if (!ako::ensure_dynamic_smem<paged_decode_kernel<T, D, FP8, ALIGNED, FOLD>>(most)) return AKO4X_ELAUNCH;
   const int smem = ringed(D, FP8) || pl.per_cta < WARPS ? most : 0;
-  paged_decode_kernel<T, D, FP8, ALIGNED, FOLD><<<(unsigned)(pl.shares * pl.unit_ctas), THREADS, smem, st>>>(p);
-  AKO_CHECK_LAUNCH();
+  if (ako::launch_pdl(true, paged_decode_kernel<T, D, FP8, ALIGNED, FOLD>, dim3((unsigned)(pl.shares * pl.unit_ctas)), dim3(THREADS), smem, st, p) !=
+      cudaSuccess)
+    return AKO4X_ELAUNCH;
   if (pl.shares == 1) return AKO4X_OK;
   const int64_t jobs = (int64_t)std::min(p.batch, p.shares) * p.q_heads;
   const bool many = p.shares >= 8LL * p.batch;      // partials of a sequence

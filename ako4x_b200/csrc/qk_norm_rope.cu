@@ -97,6 +97,8 @@ template <class T, int LANES, Partner PARTNER>
 __global__ void __launch_bounds__(WARPS * 32, PARTNER == MEMORY ? 3 : 5) qk_norm_rope_kernel(const Params p) {
   constexpr int GROUP = 32 / LANES;   // rows of a warp instruction
   __shared__ __align__(16) float2 s_cs[WARPS][MAX_DIM / 2];
+  ako::pdl_trigger();
+  ako::pdl_wait();   // nothing before this reads what a kernel wrote, and no load below is of the read-only kind
   const int warp = threadIdx.x >> 5, lane32 = threadIdx.x & 31;
   const int lane = lane32 % LANES, sub = lane32 / LANES;
   const int64_t token = (int64_t)blockIdx.x * WARPS + warp;
@@ -128,8 +130,8 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == MEMORY ? 3 : 5) qk_norm
   };
   auto fetch = [&](uint4 (&x)[2]) {
     if (at >= g1) return;
-    x[0] = __ldg(reinterpret_cast<const uint4*>(from0));
-    x[1] = __ldg(reinterpret_cast<const uint4*>(from1));
+    x[0] = *reinterpret_cast<const uint4*>(from0);
+    x[1] = *reinterpret_cast<const uint4*>(from1);
     if (++at == at_stop) {
       if (at < g1) {
         at_kind = at < end_k ? 1 : 2;
@@ -154,7 +156,7 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == MEMORY ? 3 : 5) qk_norm
   if (g0 < end_k) {
     const double pos = p.positions64 ? (double)((const int64_t*)p.positions)[token] : (double)((const int32_t*)p.positions)[token];
     for (int i = lane32; i < half; i += 32) {
-      double turn = pos * ((double)__ldg(p.inv_freq + i) * 0.15915494309189533577);   // f / 2 pi
+      double turn = pos * ((double)p.inv_freq[i] * 0.15915494309189533577);   // f / 2 pi
       turn -= rint(turn);
       // and the nearest quarter: sine and cosine are then both good to their last bits, next to their zeros too
       const double quarters = rint(turn * 4.0);
@@ -192,11 +194,11 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == MEMORY ? 3 : 5) qk_norm
         if (p.weights32) {
 #pragma unroll
           for (int j = 0; j < 8; j += 4) {
-            const float4 y = __ldg(reinterpret_cast<const float4*>((const float*)weight + e + j));
+            const float4 y = *reinterpret_cast<const float4*>((const float*)weight + e + j);
             w[h][j] = y.x, w[h][j + 1] = y.y, w[h][j + 2] = y.z, w[h][j + 3] = y.w;
           }
         } else {
-          const uint4 x = __ldg(reinterpret_cast<const uint4*>((const T*)weight + e));
+          const uint4 x = *reinterpret_cast<const uint4*>((const T*)weight + e);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float2 y = Pair<T>::get(word(x, j));
@@ -340,7 +342,7 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == MEMORY ? 3 : 5) qk_norm
                 v[c] = 0.f;
                 if (e < p.rotary) {
                   v[c] = Pair<T>::one(row + other * 2);
-                  if (weight) v[c] *= p.weights32 ? __ldg((const float*)weight + other) : Pair<T>::one((const T*)weight + other);
+                  if (weight) v[c] *= p.weights32 ? ((const float*)weight)[other] : Pair<T>::one((const T*)weight + other);
                 }
               }
               o[h][j] = f2(v[0], v[1]);
@@ -424,19 +426,15 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == MEMORY ? 3 : 5) qk_norm
 }
 
 template <class T, int LANES>
-void launch(const Params& p, dim3 blocks, cudaStream_t st) {
-  if (p.interleaved)
-    qk_norm_rope_kernel<T, LANES, SAME_PIECE><<<blocks, WARPS * 32, 0, st>>>(p);
-  else if (p.rotary % 16 == 0)
-    qk_norm_rope_kernel<T, LANES, OTHER_PIECE><<<blocks, WARPS * 32, 0, st>>>(p);
-  else
-    qk_norm_rope_kernel<T, LANES, MEMORY><<<blocks, WARPS * 32, 0, st>>>(p);
+cudaError_t launch(const Params& p, dim3 blocks, cudaStream_t st) {
+  const auto kernel = p.interleaved         ? qk_norm_rope_kernel<T, LANES, SAME_PIECE>
+                      : p.rotary % 16 == 0 ? qk_norm_rope_kernel<T, LANES, OTHER_PIECE>
+                                           : qk_norm_rope_kernel<T, LANES, MEMORY>;
+  return ako::launch_pdl(true, kernel, blocks, dim3(WARPS * 32), 0, st, p);
 }
 template <class T>
-void launch(const Params& p, int lanes, dim3 blocks, cudaStream_t st) {
-  if (lanes == 4) launch<T, 4>(p, blocks, st);
-  else if (lanes == 8) launch<T, 8>(p, blocks, st);
-  else launch<T, 16>(p, blocks, st);
+cudaError_t launch(const Params& p, int lanes, dim3 blocks, cudaStream_t st) {
+  return lanes == 4 ? launch<T, 4>(p, blocks, st) : lanes == 8 ? launch<T, 8>(p, blocks, st) : launch<T, 16>(p, blocks, st);
 }
 
 bool aligned(const void* ptr, int64_t a, int64_t b, int64_t c, int64_t to) {
@@ -483,10 +481,8 @@ int run(Params& p, const ako4x_head_rows* q, const ako4x_head_rows* k, const ako
   if (blocks > 0x7fffffffLL || shares > 65535 || groups > 0x3fffffffLL) return AKO4X_ETOOLARGE;
   const dim3 grid((unsigned)blocks, (unsigned)shares);
   cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == AKO4X_BF16) launch<__nv_bfloat16>(p, lanes, grid, st);
-  else launch<__half>(p, lanes, grid, st);
-  AKO_CHECK_LAUNCH();
-  return AKO4X_OK;
+  const cudaError_t e = dtype == AKO4X_BF16 ? launch<__nv_bfloat16>(p, lanes, grid, st) : launch<__half>(p, lanes, grid, st);
+  return e == cudaSuccess ? AKO4X_OK : AKO4X_ELAUNCH;
 }
 
 Params common(const void* positions, int positions_int64, const float* inv_freq, int interleaved, float factor, void* q_out,

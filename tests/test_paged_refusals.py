@@ -242,7 +242,7 @@ def test_pages_c_status(built_lib):
     assert L.ako4x_kv_pages_fork(one, size, short, 1, x, x, x, x, x, x, 2, 4, 4, 4, 16, x, 4096, None) == EINVAL
     assert L.ako4x_kv_pages_fork(one, size, stride, 1, x, x, x, x, x, x, 2, 4, 4, 4, 16, x, 16, None) == EWORKSPACE
     assert L.ako4x_kv_pages_copy(one, size, stride, 1, x, x, None, 2, 4, x, 4096, None) == EINVAL
-    assert L.ako4x_kv_pages_copy(one, size, stride, 1, x, x, x, 2, 4, None, 0, None) == EWORKSPACE
+    assert L.ako4x_kv_pages_copy(one, size, stride, 1, x, x, x, 5000, 4, None, 0, None) == EWORKSPACE
     assert L.ako4x_kv_pages_compact(one, size, stride, 1, x, x, x, 4, 4, 0, None, 0, None) == OK
     assert L.ako4x_kv_pages_compact(one, size, stride, 1, x, x, x, 4, 4, 4, None, 0, None) == EWORKSPACE
     assert L.ako4x_kv_pages_compact(one, size, stride, 1, x, x, x, -4, 4, 4, x, 4096, None) == EINVAL
