@@ -92,9 +92,6 @@ __device__ __forceinline__ uint4 ld16(const uint4* p) {
   asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
   return r;
 }
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(dst), "l"(src) : "memory");
-}
 __device__ __forceinline__ uint4 lds16(uint32_t a) {
   uint4 r;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
@@ -172,20 +169,17 @@ __device__ __forceinline__ void empty_head(const Params& p, int64_t row_head) { 
   p.lse[row_head] = -INFINITY;
 }
 
-// Where the tiles under way are: in registers, one of K and one of V, or (e4m3, which takes so long to work on that more
-// of them are needed, and 256 features, which are too many registers) in shared memory, some per warp.
+// Where the tiles under way are: K in registers; V too, or (e4m3, whose work on a tile is a long chain, and 256
+// features, which are too many registers) two tiles of it in shared memory. Not K as well: an SM takes a 512-byte
+// asynchronous copy every 20 cycles or so, which is 5.6 TB/s for the GPU.
 __host__ __device__ constexpr bool ringed(int64_t d, bool fp8) { return fp8 || d == 256; }
-__host__ __device__ constexpr int ctas_per_sm(int64_t, bool) { return 3; }
-// Blocks of a tile: two in e4m3 (64 and 128 features), whose work on a block is a long chain.
+__host__ __device__ constexpr int ctas_per_sm(int64_t d, bool fp8) { return d == 256 && !fp8 ? 2 : 3; }
+// Blocks of a tile: two in e4m3 (64 and 128 features).
 __host__ __device__ constexpr int blocks(int64_t d, bool fp8) { return fp8 && d <= 128 ? 2 : 1; }
-__host__ __device__ constexpr int depth(int64_t d, bool fp8) { return fp8 ? (d == 64 ? 3 : 2) : 1; }
-// Bytes of shared memory of a warp: K and V of its tiles, and the scales of their tokens (a quad of lanes: K's two, V's
-// two, for each block).
-__host__ __device__ constexpr int ring_bytes(int64_t d, bool fp8) {
-  return ringed(d, fp8) ? depth(d, fp8) * blocks(d, fp8) * (int)(2 * BLOCK * d * (fp8 ? 1 : 2) + (fp8 ? 128 : 0)) : 0;
-}
-// What a warp leaves for the others of its CTA: (m, l) of 8 heads, then O.
+// Shared memory of a warp: V of two tiles; and what it leaves for the others of its CTA, (m, l) of 8 heads, then O.
+__host__ __device__ constexpr int ring_bytes(int64_t d, bool fp8) { return ringed(d, fp8) ? 2 * blocks(d, fp8) * BLOCK * (int)d * (fp8 ? 1 : 2) : 0; }
 __host__ __device__ constexpr int part_bytes(int64_t d) { return (8 * (int)d + 16) * 4; }
+__host__ __device__ constexpr int warp_bytes(int64_t d, bool fp8) { return ring_bytes(d, fp8) > part_bytes(d) ? ring_bytes(d, fp8) : part_bytes(d); }
 
 template <class T, int D, bool FP8, bool ALIGNED, bool FOLD>
 __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_kernel(const Params p) {
@@ -194,12 +188,11 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
   constexpr int KS = D / 16;                       // steps of 16 features
   constexpr bool RINGED = ringed(D, FP8);
   constexpr int TT = blocks(D, FP8), TILE = BLOCK * TT, R = 2 * TT;   // R: tokens of a lane in a tile
-  constexpr int DEPTH = depth(D, FP8), RING = ring_bytes(D, FP8), HALF = R * NJ * 512;   // HALF: K, or V, of a tile
-  constexpr int PART = RINGED ? RING : part_bytes(D);
+  constexpr int SLOT = R * NJ * 512, PART = warp_bytes(D, FP8);      // V of a tile; what a warp has of shared memory
   using TM = typename std::conditional<FP8, __half, T>::type;   // operand type
   constexpr float LIFT = std::is_same<TM, __half>::value ? 15.f : 0.f;
   __shared__ int s_scan[6];
-  extern __shared__ __align__(16) unsigned char s_ring[];   // [warp]: tiles, the scales of each; then its part
+  extern __shared__ __align__(16) unsigned char s_ring[];   // [warp]: its tiles, and then its part
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   ako::pdl_trigger();
@@ -221,7 +214,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
   int2 cut = cut_entry(0, 0, 0);
   int left = sh0.left, b = sh0.row, skip = sh0.skip;
 
-  const uint32_t ring = ako::smem_u32(s_ring) + warp * RING + lane * 16;
+  const uint32_t ring = ako::smem_u32(s_ring) + warp * PART + lane * 16;
   const uint4 *kbase[ALIGNED ? 2 : 1], *vbase[ALIGNED ? 2 : 1];       // ALIGNED: of tokens g and g + 8 of a tile
 #pragma unroll
   for (int i = 0; i < (ALIGNED ? 2 : 1); ++i) {
@@ -260,56 +253,52 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
         id[i] = pages[page];
       }
     };
-    uint64_t voff[IDS];
-    uint32_t seen = 0;                              // R bits for each tile under way, the oldest on top
-    // Copies under way: K and V of a tile are a group each, in the order in which they are needed. A lane copies what
-    // it will read itself, so waiting for its own copies is all it takes.
-    uint4 kc[RINGED ? 1 : R][RINGED ? 1 : NJ], vc[RINGED ? 1 : R][RINGED ? 1 : NJ];
-    float scn[TT];
-    auto request_k = [&](int tile, uint32_t to) {
-      seen <<= R;
-      if (tile < te) {
-        uint64_t off[IDS];
-        bool real[IDS];
+    // A tile's offsets, and R bits that say which of this lane's tokens are visible
+    uint64_t koff[IDS], voff[IDS], soff[TT];
+    uint32_t bits = 0, seen = 0;
+    auto locate = [&](int tile) {
+      bool real[IDS];
 #pragma unroll
-        for (int i = 0; i < IDS; ++i) {
-          real[i] = (unsigned)id[i] < (unsigned)p.num_pages;
-          const uint32_t page = real[i] ? id[i] : 0, sl = slot[i];
-          off[i] = (uint64_t)page * p.k.page + sl * p.k.slot;
-          voff[i] = p.same_strides ? off[i] : (uint64_t)page * p.v.page + sl * p.v.slot;
-          if (FP8 && (ALIGNED || (i & 1) == (t & 1))) {
-            const float* from = sc_base + ((uint64_t)page * sc_page + sl * sc_slot);
-            if (RINGED) cp_async4(to - lane * 12 + 2 * HALF + (ALIGNED ? i : i / 2) * 128, from);
-            else scn[ALIGNED ? i : i / 2] = *from;
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-          const int tok = (tile0 + tile) * TILE + 8 * i + g;
-          seen |= (uint32_t)(real[ALIGNED ? i / 2 : i] && tok >= sp.lo && tok < sp.hi) << i;
-          const uint4* from = kbase[ALIGNED ? i & 1 : 0] + off[ALIGNED ? i / 2 : i];
-#pragma unroll
-          for (int j = 0; j < NJ; ++j) {
-            if (RINGED) ako::cp_async16(to + (i * NJ + j) * 512, from + 4 * j);
-            else kc[RINGED ? 0 : i][RINGED ? 0 : j] = ld16(from + 4 * j);
-          }
-        }
+      for (int i = 0; i < IDS; ++i) {
+        real[i] = (unsigned)id[i] < (unsigned)p.num_pages;
+        const uint32_t page = real[i] ? id[i] : 0, sl = slot[i];
+        koff[i] = (uint64_t)page * p.k.page + sl * p.k.slot;
+        voff[i] = p.same_strides ? koff[i] : (uint64_t)page * p.v.page + sl * p.v.slot;
+        if (FP8 && (ALIGNED || (i & 1) == (t & 1))) soff[ALIGNED ? i : i / 2] = (uint64_t)page * sc_page + sl * sc_slot;
       }
-      if (RINGED) ako::cp_async_commit();
+      bits = 0;
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        const int tok = (tile0 + tile) * TILE + 8 * i + g;
+        bits |= (uint32_t)(real[ALIGNED ? i / 2 : i] && tok >= sp.lo && tok < sp.hi) << i;
+      }
     };
-    auto request_v = [&](int tile, uint32_t to) {
-      if (tile < te) {
+    uint4 kc[R][NJ], vc[RINGED ? 1 : R][RINGED ? 1 : NJ];
+    float scales[TT];                               // of the quad's token that is this lane's
+    auto request_k = [&] {
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
-          const uint4* from = vbase[ALIGNED ? i & 1 : 0] + voff[ALIGNED ? i / 2 : i];
+      for (int i = 0; i < R; ++i) {
+        const uint4* from = kbase[ALIGNED ? i & 1 : 0] + koff[ALIGNED ? i / 2 : i];
 #pragma unroll
-          for (int j = 0; j < NJ; ++j) {
-            if (RINGED) ako::cp_async16(to + HALF + (i * NJ + j) * 512, from + 4 * j);
-            else vc[RINGED ? 0 : i][RINGED ? 0 : j] = ld16(from + 4 * j);
-          }
+        for (int j = 0; j < NJ; ++j) kc[i][j] = ld16(from + 4 * j);
+      }
+      if (FP8) {
+#pragma unroll
+        for (int u = 0; u < TT; ++u) scales[u] = sc_base[soff[u]];
+      }
+      seen = bits;
+    };
+    // A lane copies what it will read itself, so waiting for its own copies is all it takes.
+    auto request_v = [&](uint32_t to) {
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        const uint4* from = vbase[ALIGNED ? i & 1 : 0] + voff[ALIGNED ? i / 2 : i];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          if (RINGED) ako::cp_async16(to + (i * NJ + j) * 512, from + 4 * j);
+          else vc[RINGED ? 0 : i][RINGED ? 0 : j] = ld16(from + 4 * j);
         }
       }
-      if (RINGED) ako::cp_async_commit();
     };
 
     // q of the block's heads as B fragments (n = head g), in the order of the K pieces. FOLD: the columns 4 to 7
@@ -372,33 +361,44 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
     // The maxima start at the lowest finite value, so that a score of -inf weighs 0 whatever else there is.
     float m0 = -FLT_MAX, m1 = -FLT_MAX, l0 = 0.f, l1 = 0.f;
 
-    // slots of the ring: this one's address, each 2 HALF (+ 512) bytes
-    constexpr uint32_t SLOT = RING / DEPTH;
+    // K is asked for a tile ahead of the work, V one (registers) or two (shared memory), page ids one ahead of that. V in
+    // shared memory is a group of copies for each tile, an empty one where there is none.
+    const int begin = skip + my;
     uint32_t at_slot = ring;
-    int ids[DEPTH][IDS], slots[DEPTH][IDS];
+    if (begin < te) {
+      fetch_ids(begin);
+      int id0[IDS], slot0[IDS];
 #pragma unroll
-    for (int d = 0; d < DEPTH; ++d) {
-      if (skip + my + d * along < te) fetch_ids(skip + my + d * along);
+      for (int i = 0; i < IDS; ++i) id0[i] = id[i], slot0[i] = slot[i];
+      if (begin + along < te) fetch_ids(begin + along);   // under way with the first ones
 #pragma unroll
-      for (int i = 0; i < IDS; ++i) ids[d][i] = id[i], slots[d][i] = slot[i];
+      for (int i = 0; i < IDS; ++i) {
+        const int a = id[i], b = slot[i];
+        id[i] = id0[i], slot[i] = slot0[i];
+        id0[i] = a, slot0[i] = b;
+      }
+      locate(begin);
+      request_k();
+      request_v(ring);
+#pragma unroll
+      for (int i = 0; i < IDS; ++i) id[i] = id0[i], slot[i] = slot0[i];
     }
-#pragma unroll
-    for (int d = 0; d < DEPTH; ++d) {
-#pragma unroll
-      for (int i = 0; i < IDS; ++i) id[i] = ids[d][i], slot[i] = slots[d][i];
-      request_k(skip + my + d * along, ring + d * SLOT);
-      request_v(skip + my + d * along, ring + d * SLOT);
+    if (RINGED) {
+      ako::cp_async_commit();
+      if (begin + along < te) {
+        locate(begin + along);
+        request_v(ring + SLOT);
+      }
+      ako::cp_async_commit();
+      if (begin + 2 * along < te) fetch_ids(begin + 2 * along);
     }
-    if (skip + my + DEPTH * along < te) fetch_ids(skip + my + DEPTH * along);
-    for (int tile = skip + my; tile < te; tile += along) {
-      if (RINGED) ako::cp_async_wait<2 * DEPTH - 1>();
+    for (int tile = begin; tile < te; tile += along) {
       float s[TT][2][4] = {};                        // two chains of products for a block, joined below
 #pragma unroll
       for (int j = 0; j < NJ; ++j)
 #pragma unroll
         for (int u = 0; u < TT; ++u) {
-          const uint4 x = RINGED ? lds16(at_slot + (2 * u * NJ + j) * 512) : kc[RINGED ? 0 : 2 * u][RINGED ? 0 : j];
-          const uint4 y = RINGED ? lds16(at_slot + ((2 * u + 1) * NJ + j) * 512) : kc[RINGED ? 0 : 2 * u + 1][RINGED ? 0 : j];
+          const uint4 &x = kc[2 * u][j], &y = kc[2 * u + 1][j];
           if (FP8) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -415,27 +415,23 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
         }
       float ks[R], vs[R];
       if (FP8) {
-        if (RINGED) __syncwarp();                    // the quad's copies have arrived
 #pragma unroll
-        for (int u = 0; u < TT; ++u) {
-          if (!RINGED) {
-            ks[2 * u] = __shfl_sync(0xffffffffu, scn[u], lane & ~3), ks[2 * u + 1] = __shfl_sync(0xffffffffu, scn[u], lane & ~3 | 1);
-            vs[2 * u] = __shfl_sync(0xffffffffu, scn[u], lane & ~3 | 2), vs[2 * u + 1] = __shfl_sync(0xffffffffu, scn[u], lane | 3);
-            continue;
-          }
-          const uint4 x = lds16(at_slot - lane * 16 + 2 * HALF + u * 128 + (lane & ~3) * 4);
-          ks[2 * u] = __uint_as_float(x.x), ks[2 * u + 1] = __uint_as_float(x.y);
-          vs[2 * u] = __uint_as_float(x.z), vs[2 * u + 1] = __uint_as_float(x.w);
+        for (int u = 0; u < TT; ++u) {               // t = 0, 1: K's two, t = 2, 3: V's
+          ks[2 * u] = __shfl_sync(0xffffffffu, scales[u], lane & ~3), ks[2 * u + 1] = __shfl_sync(0xffffffffu, scales[u], (lane & ~3) | 1);
+          vs[2 * u] = __shfl_sync(0xffffffffu, scales[u], (lane & ~3) | 2), vs[2 * u + 1] = __shfl_sync(0xffffffffu, scales[u], lane | 3);
         }
-        if (RINGED) __syncwarp();                    // and been read before the next ones
       }
       bool now[R], all = true;
 #pragma unroll
       for (int i = 0; i < R; ++i) {
-        now[i] = (seen >> (R * (DEPTH - 1) + i) & 1) != 0;
+        now[i] = (seen >> i & 1) != 0;
         all &= now[i];
       }
-      request_k(tile + DEPTH * along, at_slot);
+      const bool more = tile + along < te;
+      if (more) {
+        if (!RINGED) locate(tile + along);
+        request_k();
+      }
       // a lane's tokens, heads 2t and 2t + 1
       float e[R][2];
       float n0 = -INFINITY, n1 = -INFINITY;
@@ -472,14 +468,14 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
         l0 += e[i][0];
         l1 += e[i][1];
       }
-      if (RINGED) ako::cp_async_wait<2 * DEPTH - 1>();
+      if (RINGED) ako::cp_async_wait<1>();
       if (!all) {   // weight 0, but what was read in its place may hold anything
 #pragma unroll
         for (int i = 0; i < R; ++i)
 #pragma unroll
           for (int j = 0; j < NJ; ++j)
             if (!now[i]) {
-              if (RINGED) sts16(at_slot + HALF + (i * NJ + j) * 512, make_uint4(0u, 0u, 0u, 0u));
+              if (RINGED) sts16(at_slot + (i * NJ + j) * 512, make_uint4(0u, 0u, 0u, 0u));
               else vc[RINGED ? 0 : i][RINGED ? 0 : j] = make_uint4(0u, 0u, 0u, 0u);
             }
       }
@@ -528,8 +524,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
       for (int j = 0; j < NJ; ++j)
 #pragma unroll
         for (int u = 0; u < TT; ++u) {
-          const uint4 x = RINGED ? lds16(at_slot + HALF + (2 * u * NJ + j) * 512) : vc[RINGED ? 0 : 2 * u][RINGED ? 0 : j];
-          const uint4 y = RINGED ? lds16(at_slot + HALF + ((2 * u + 1) * NJ + j) * 512) : vc[RINGED ? 0 : 2 * u + 1][RINGED ? 0 : j];
+          const uint4 x = RINGED ? lds16(at_slot + (2 * u * NJ + j) * 512) : vc[RINGED ? 0 : 2 * u][RINGED ? 0 : j];
+          const uint4 y = RINGED ? lds16(at_slot + ((2 * u + 1) * NJ + j) * 512) : vc[RINGED ? 0 : 2 * u + 1][RINGED ? 0 : j];
 #pragma unroll
           for (int i = 0; i < (FP8 ? 4 : 2); ++i) {
             uint32_t x0, x1, y0, y1;
@@ -545,11 +541,17 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
             mma<TM>(d, a, bh[2 * u], bh[2 * u + 1]);
           }
         }
-      request_v(tile + DEPTH * along, at_slot);
-      if (tile + (DEPTH + 1) * along < te) fetch_ids(tile + (DEPTH + 1) * along);
       if (RINGED) {
-        at_slot += SLOT;
-        if (at_slot == ring + RING) at_slot = ring;
+        if (tile + 2 * along < te) {
+          locate(tile + 2 * along);
+          request_v(at_slot);
+        }
+        ako::cp_async_commit();
+        if (tile + 3 * along < te) fetch_ids(tile + 3 * along);
+        at_slot = at_slot == ring ? ring + SLOT : ring;
+      } else if (more) {
+        request_v(0);
+        if (tile + 2 * along < te) fetch_ids(tile + 2 * along);
       }
     }
 #pragma unroll
@@ -669,7 +671,6 @@ __global__ void __launch_bounds__(128) paged_merge_few_kernel(const Params p) {
   constexpr int C = D / 32;                         // columns per lane
   const int lane = threadIdx.x & 31;
   const int64_t job = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  ako::pdl_trigger();
   ako::pdl_wait();
   if (job >= (int64_t)min(p.batch, p.shares) * p.q_heads) return;
   const int head = (int)(job % p.q_heads);
@@ -722,7 +723,6 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) paged_merge_many_kernel(cons
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int block = blockIdx.x % (D / 64);
   const int64_t job = blockIdx.x / (D / 64);
-  ako::pdl_trigger();
   ako::pdl_wait();
   const int head = (int)(job % p.q_heads);
   const Cut cut(p, job / p.q_heads);
@@ -804,8 +804,7 @@ inline Plan plan_for(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t d
 }
 template <class T, int D, bool FP8, bool ALIGNED, bool FOLD>
 int launch(const Params& p, const Plan& pl, cudaStream_t st) {
-  constexpr int most = WARPS * (ringed(D, FP8) ? ring_bytes(D, FP8) : part_bytes(D));
-  static_assert(!ringed(D, FP8) || ring_bytes(D, FP8) >= part_bytes(D), "a warp's part is put where its tiles were");
+  constexpr int most = WARPS * warp_bytes(D, FP8);
   if (!ako::ensure_dynamic_smem<paged_decode_kernel<T, D, FP8, ALIGNED, FOLD>>(most)) return AKO4X_ELAUNCH;
   const int smem = ringed(D, FP8) || pl.per_cta < WARPS ? most : 0;
   if (ako::launch_pdl(true, paged_decode_kernel<T, D, FP8, ALIGNED, FOLD>, dim3((unsigned)(pl.shares * pl.unit_ctas)), dim3(THREADS), smem, st, p) !=
