@@ -28,7 +28,9 @@
 namespace {
 
 constexpr int WARPS = 4;
+constexpr int WARPS_TO_FILL = 20;   // of an SM
 constexpr int MAX_DIM = 256;
+constexpr int MAX_ANGLES = 256;   // of a warp: 256 / dim tokens at most, half of dim each, and room for odd numbers
 
 struct Rows {                 // heads of one kind
   const unsigned char* in;
@@ -55,6 +57,7 @@ struct Params {
   int64_t tokens, num_slots;
   int dim, rotary, page_size;
   int per_share;              // groups of a warp
+  int log_tokens;             // tokens of a warp, side by side
   float eps, inv_dim, factor;
   bool interleaved, positions64, slots64, weights32, quant, ragged;   // ragged: some lanes are behind the row's end
 };
@@ -96,18 +99,21 @@ enum Partner { OTHER_PIECE, SAME_PIECE, MEMORY };
 template <class T, int LANES, Partner PARTNER>
 __global__ void __launch_bounds__(WARPS * 32, PARTNER == MEMORY ? 3 : 5) qk_norm_rope_kernel(const Params p) {
   constexpr int GROUP = 32 / LANES;   // rows of a warp instruction
-  __shared__ __align__(16) float2 s_cs[WARPS][MAX_DIM / 2];
+  __shared__ __align__(16) float2 s_cs[WARPS][MAX_ANGLES];
   ako::pdl_trigger();
   ako::pdl_wait();   // nothing before this reads what a kernel wrote, and no load below is of the read-only kind
   const int warp = threadIdx.x >> 5, lane32 = threadIdx.x & 31;
-  const int lane = lane32 % LANES, sub = lane32 / LANES;
-  const int64_t token = (int64_t)blockIdx.x * WARPS + warp;
-  if (token >= p.tokens) return;      // whole warps; there is no block barrier
+  const int lane = lane32 % LANES, slots = GROUP >> p.log_tokens;   // slots: rows of a token at once
+  const int sub = lane32 / LANES & (slots - 1), mine = lane32 / LANES / slots;
+  const int64_t first = ((int64_t)blockIdx.x * WARPS + warp) << p.log_tokens;
+  if (first >= p.tokens) return;      // whole warps; there is no block barrier
+  const int64_t token = min(first + mine, p.tokens - 1);
+  const bool real = first + mine < p.tokens;
   const int end_q = p.q.groups, end_k = end_q + p.k.groups, end_v = end_k + p.v.groups;
   const int g0 = blockIdx.y * p.per_share, g1 = min(g0 + p.per_share, end_v);
 
   // this lane's two pieces of a row: the partners of each other in front, neighbours behind
-  const int half = p.rotary / 2, paired = PARTNER == OTHER_PIECE ? p.rotary / 16 : 0;
+  const int half = p.rotary / 2, pitch = (half + 1) & ~1, paired = PARTNER == OTHER_PIECE ? p.rotary / 16 : 0;
   const int e0 = 8 * (lane < paired ? lane : 2 * lane), e1 = 8 * (lane < paired ? lane + paired : 2 * lane + 1);
   const bool in0 = e0 < p.dim, in1 = e1 < p.dim;
 
@@ -121,12 +127,12 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == MEMORY ? 3 : 5) qk_norm
     const Rows& r = at_kind == 0 ? p.q : at_kind == 1 ? p.k : p.v;
     const int start = at_kind == 0 ? 0 : at_kind == 1 ? end_q : end_k;
     at_stop = min(g1, start + r.groups);
-    at_head = (at - start) * GROUP + sub;
+    at_head = (at - start) * slots + sub;
     at_heads = r.heads;
     from0 = r.in + token * r.token_stride + min(at_head, at_heads - 1) * r.head_stride;
     from1 = from0 + (in1 ? e1 * 2 : 0);
     from0 += in0 ? e0 * 2 : 0;
-    step = GROUP * r.head_stride;
+    step = slots * r.head_stride;
   };
   auto fetch = [&](uint4 (&x)[2]) {
     if (at >= g1) return;
@@ -138,7 +144,7 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == MEMORY ? 3 : 5) qk_norm
         aim();
       }
     } else {
-      at_head += GROUP;
+      at_head += slots;
       if (at_head < at_heads) {
         from0 += step;
         from1 += step;
@@ -154,17 +160,19 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == MEMORY ? 3 : 5) qk_norm
   };
 
   if (g0 < end_k) {
-    const double pos = p.positions64 ? (double)((const int64_t*)p.positions)[token] : (double)((const int32_t*)p.positions)[token];
-    for (int i = lane32; i < half; i += 32) {
-      double turn = pos * ((double)p.inv_freq[i] * 0.15915494309189533577);   // f / 2 pi
-      turn -= rint(turn);
-      // and the nearest quarter: sine and cosine are then both good to their last bits, next to their zeros too
-      const double quarters = rint(turn * 4.0);
-      float s, c;
-      sincospif(2.0f * (float)(turn - quarters * 0.25), &s, &c);
-      const int quadrant = (int)quarters & 3;
-      const float x = quadrant & 1 ? -s : c, y = quadrant & 1 ? c : s;
-      s_cs[warp][i] = make_float2((quadrant & 2 ? -x : x) * p.factor, (quadrant & 2 ? -y : y) * p.factor);
+    for (int t = 0; t < 1 << p.log_tokens && first + t < p.tokens; ++t) {
+      const double pos = p.positions64 ? (double)((const int64_t*)p.positions)[first + t] : (double)((const int32_t*)p.positions)[first + t];
+      for (int i = lane32; i < half; i += 32) {
+        double turn = pos * ((double)p.inv_freq[i] * 0.15915494309189533577);   // f / 2 pi
+        turn -= rint(turn);
+        // and the nearest quarter: sine and cosine are then both good to their last bits, next to their zeros too
+        const double quarters = rint(turn * 4.0);
+        float s, c;
+        sincospif(2.0f * (float)(turn - quarters * 0.25), &s, &c);
+        const int quadrant = (int)quarters & 3;
+        const float x = quadrant & 1 ? -s : c, y = quadrant & 1 ? c : s;
+        s_cs[warp][t * pitch + i] = make_float2((quadrant & 2 ? -x : x) * p.factor, (quadrant & 2 ? -y : y) * p.factor);
+      }
     }
     __syncwarp();
   }
@@ -180,6 +188,7 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == MEMORY ? 3 : 5) qk_norm
     }
   }
 
+  const float2* cs_of = s_cs[warp] + (real ? mine : 0) * pitch;
   // Pairs (2i, 2i + 1) of the pieces' elements: z = inv (x A + x' B), where `mask` says so; inv x A elsewhere.
   F2 A[2][4], B[2][4];
   unsigned mask = 0;
@@ -219,7 +228,7 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == MEMORY ? 3 : 5) qk_norm
         mask = 0xffu;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float4 cs = *reinterpret_cast<const float4*>(&s_cs[warp][e0 + 2 * j]);
+          const float4 cs = *reinterpret_cast<const float4*>(cs_of + e0 + 2 * j);
           A[0][j] = f2(w[0][2 * j] * cs.x, w[0][2 * j + 1] * cs.z);
           A[1][j] = f2(w[1][2 * j] * cs.x, w[1][2 * j + 1] * cs.z);
           B[0][j] = f2(-w[1][2 * j] * cs.y, -w[1][2 * j + 1] * cs.w);
@@ -233,7 +242,7 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == MEMORY ? 3 : 5) qk_norm
         for (int j = 0; j < 4; ++j) {
           const int e = (h ? e1 : e0) + 2 * j;
           if (e < p.rotary) {
-            const float2 cs = s_cs[warp][e / 2];
+            const float2 cs = cs_of[e / 2];
             mask |= 1u << (4 * h + j);
             A[h][j] = f2(w[h][2 * j] * cs.x, w[h][2 * j + 1] * cs.x);
             B[h][j] = f2(-w[h][2 * j + 1] * cs.y, w[h][2 * j] * cs.y);
@@ -249,7 +258,7 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == MEMORY ? 3 : 5) qk_norm
           for (int c = 0; c < 2; ++c) {
             const int e = (h ? e1 : e0) + 2 * j + c;
             if (e < p.rotary) {
-              const float2 cs = s_cs[warp][e < half ? e : e - half];
+              const float2 cs = cs_of[e < half ? e : e - half];
               a[c] *= cs.x;
               b[c] = e < half ? -cs.y : cs.y;
             }
@@ -267,7 +276,7 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == MEMORY ? 3 : 5) qk_norm
     const int kind = it < end_q ? 0 : it < end_k ? 1 : 2, start = kind == 0 ? 0 : kind == 1 ? end_q : end_k;
     const Rows& r = kind == 0 ? p.q : kind == 1 ? p.k : p.v;
     const int heads = r.heads, stop = min(g1, start + r.groups);
-    int head = (it - start) * GROUP + sub;
+    int head = (it - start) * slots + sub;
     const bool to_cache = kind == 2 || (kind == 1 && !p.k_out), turn = kind != 2;
     const void* weight = kind == 0 ? p.q_weight : kind == 1 ? p.k_weight : nullptr;
     if (turn && (weight || !ready)) {
@@ -281,21 +290,21 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == MEMORY ? 3 : 5) qk_norm
     const bool quant = to_cache && p.quant;
     if (!to_cache) {
       out = (kind == 0 ? p.q_out : p.k_out) + (token * heads + head) * p.dim * 2;
-      out_step = (int64_t)GROUP * p.dim * 2;
+      out_step = (int64_t)slots * p.dim * 2;
     } else {
       const Cache& c = kind == 1 ? p.kc : p.vc;
       out = c.data + page * c.page_stride + slot * c.slot_stride + head * c.head_stride;
-      out_step = GROUP * c.head_stride;
+      out_step = slots * c.head_stride;
       if (quant) {
         scale_out = c.scale + page * c.scale_page_stride + slot * c.scale_slot_stride + head * c.scale_head_stride;
-        scale_step = GROUP * c.scale_head_stride;
+        scale_step = slots * c.scale_head_stride;
       }
     }
     unsigned char *to0 = out + (quant ? e0 : e0 * 2), *to1 = out + (quant ? e1 : e1 * 2);
-    const bool store = !to_cache || stored;
+    const bool store = real && (!to_cache || stored);
     if (!turn && !quant) {            // values as they are
 #pragma unroll 1
-      for (; it < stop; ++it, head += GROUP, to0 += out_step, to1 += out_step) {
+      for (; it < stop; ++it, head += slots, to0 += out_step, to1 += out_step) {
         const uint4 x0 = raw[0][0], x1 = raw[0][1];
         next();
         if (store && head < heads && in0) __stcs(reinterpret_cast<uint4*>(to0), x0);
@@ -303,7 +312,7 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == MEMORY ? 3 : 5) qk_norm
       }
     }
 #pragma unroll 1
-    for (; it < stop; ++it, head += GROUP, to0 += out_step, to1 += out_step) {
+    for (; it < stop; ++it, head += slots, to0 += out_step, to1 += out_step) {
       const bool live = store && head < heads;
       F2 y[2][4];
 #pragma unroll
@@ -450,7 +459,7 @@ int run(Params& p, const ako4x_head_rows* q, const ako4x_head_rows* k, const ako
   const int group = 32 / lanes;
   const ako4x_head_rows* in[3] = {q, k, v};
   Rows* to[3] = {&p.q, &p.k, &p.v};
-  int64_t groups = 0;
+  bool any = false;
   for (int i = 0; i < 3; ++i) {
     *to[i] = Rows{};
     if (!in[i]) continue;
@@ -461,10 +470,9 @@ int run(Params& p, const ako4x_head_rows* q, const ako4x_head_rows* k, const ako
     to[i]->token_stride = in[i]->token_stride * 2;
     to[i]->head_stride = in[i]->head_stride * 2;
     to[i]->heads = (int)in[i]->heads;
-    to[i]->groups = (int)ako::cdiv(in[i]->heads, group);
-    groups += to[i]->groups;
+    any = true;
   }
-  if (tokens == 0 || groups == 0) return AKO4X_OK;
+  if (!any) return AKO4X_OK;
   if (!p.positions || (rotary && !p.inv_freq)) return AKO4X_EINVAL;
   if (p.q.heads && !aligned(p.q_out, 0, 0, 0, 16)) return AKO4X_EINVAL;
   p.tokens = tokens;
@@ -472,12 +480,22 @@ int run(Params& p, const ako4x_head_rows* q, const ako4x_head_rows* k, const ako
   p.rotary = (int)rotary;
   p.inv_dim = 1.0f / (float)dim;
   p.ragged = dim != lanes * 16;
-  // A warp takes a token's rows, or a share of them while there are fewer warps than the GPU holds.
+  // A warp takes a token's rows; several tokens side by side, as long as there are warps for the GPU, where a token has few
+  // (what is done once for a token weighs more then: 8 192 tokens of 17 rows of 64 12.8 -> 11.3 us; with 48 rows of 128
+  // 44.7 -> 51.6, the warps are fewer and longer); or a share of the rows while there are fewer warps than the GPU holds.
+  int64_t row_groups = 0;
+  for (const Rows* r : to) row_groups += ako::cdiv(r->heads, group);
+  while (row_groups <= 4 && (group >> p.log_tokens) > 1 && (tokens >> (p.log_tokens + 1)) >= ako::sm_count() * WARPS_TO_FILL) ++p.log_tokens;
+  int64_t groups = 0;
+  for (Rows* r : to) {
+    r->groups = (int)ako::cdiv(r->heads, group >> p.log_tokens);
+    groups += r->groups;
+  }
   const int64_t wanted = (int64_t)ako::sm_count() * 32;
   int64_t shares = std::min(ako::cdiv(wanted, tokens), groups);
   p.per_share = (int)ako::cdiv(groups, shares);
   shares = ako::cdiv(groups, (int64_t)p.per_share);
-  const int64_t blocks = ako::cdiv(tokens, (int64_t)WARPS);
+  const int64_t blocks = ako::cdiv(tokens, (int64_t)WARPS << p.log_tokens);
   if (blocks > 0x7fffffffLL || shares > 65535 || groups > 0x3fffffffLL) return AKO4X_ETOOLARGE;
   const dim3 grid((unsigned)blocks, (unsigned)shares);
   cudaStream_t st = (cudaStream_t)stream;
