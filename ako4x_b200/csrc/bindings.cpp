@@ -632,6 +632,7 @@ bool check_weights(const char* op, Tensor& qw, Tensor& kw, const Tensor& q) {
     fp32 = w->scalar_type() == at::kFloat;
     any = true;
     *w = dense(*w);
+    if ((uintptr_t)w->data_ptr() & 15) *w = w->clone();   // a view into something else: the kernels read 16 bytes at once
   }
   return fp32;
 }
@@ -788,7 +789,9 @@ PyObject* paged_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
        "paged_decode: block_table int32 [batch, max_pages], seq_lens int32 [batch]");
   need(window >= 0, "paged_decode: window must be 0 (none) or a number of tokens");
   OneDevice dev(op, {&q0, &kc, &vc, &table0, &lens0, &ks, &vs});
-  const Tensor q = dense(q0), table = dense(table0), lens = dense(lens0);
+  Tensor q = dense(q0);
+  if ((uintptr_t)q.data_ptr() & 15) q = q.clone();   // a view into something else: the kernels read 16 bytes at once
+  const Tensor table = dense(table0), lens = dense(lens0);
   const int64_t max_pages = table.size(1);
   Tensor o = empty(q.sizes(), q.scalar_type(), q), lse = empty({batch, hq}, at::kFloat, q);
   Workspace ws(ako4x_paged_decode_workspace_bytes(batch, hq, hk, dim, max_pages, page_size, window), q);

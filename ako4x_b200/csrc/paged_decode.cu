@@ -56,7 +56,7 @@ extern "C" int ako4x_paged_decode(const void* q, const ako4x_kv_cache* k_cache, 
   if (!sizes_ok(batch, q_heads, kv_heads, dim, max_pages, page_size, window)) return AKO4X_EUNSUPPORTED_SHAPE;
   if (batch == 0) return AKO4X_OK;
   if (!q || !k_cache || !v_cache || !seq_lens || !o || !lse || (max_pages > 0 && !block_table)) return AKO4X_EINVAL;
-  if (((uintptr_t)q | (uintptr_t)o) & 15) return AKO4X_EINVAL;
+  if ((((uintptr_t)q | (uintptr_t)o) & 15) || (((uintptr_t)block_table | (uintptr_t)seq_lens | (uintptr_t)lse) & 3)) return AKO4X_EINVAL;
   const bool fp8 = cache_dtype == AKO4X_E4M3;
   Params p = {};
   if ((!set_cache(p.k, k_cache, fp8, kv_heads, page_size) || !set_cache(p.v, v_cache, fp8, kv_heads, page_size)) && num_pages > 0)

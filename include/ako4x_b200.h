@@ -362,7 +362,7 @@ int ako4x_rope(const ako4x_head_rows* q, const ako4x_head_rows* k, const void* p
                const float* inv_freq, int64_t rotary_dim, int interleaved, float attention_factor, void* q_out,
                void* k_out, int64_t tokens, int64_t dim, int dtype, void* stream);
 /* The same behind an RMS norm of every head in the same pass: x * rsqrt(mean(x^2) + eps) * weight over
- * dim; weights of the rows' type or fp32, [dim]. */
+ * dim; weights of the rows' type or fp32, [dim], 16-byte aligned. */
 int ako4x_qk_norm_rope(const ako4x_head_rows* q, const ako4x_head_rows* k, const void* q_weight,
                        const void* k_weight, int weights_fp32, float eps, const void* positions, int positions_int64,
                        const float* inv_freq, int64_t rotary_dim, int interleaved, float attention_factor,

@@ -160,6 +160,40 @@ def test_more_caches_than_a_launch_takes(built_lib):
         assert torch.equal(a, b.cpu())
 
 
+def test_a_cache_of_one_number_per_page_and_one_page(built_lib):
+    a, b = torch.arange(9., device="cuda"), torch.randn(9, 4, 6, device="cuda").transpose(1, 2)
+    want = b.clone()
+    want[7] = want[2]
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32).cuda()  # noqa: E731
+    assert kv_pages.copy([a, b], i32(2), i32(7)).tolist() == [True]
+    assert a[7] == 2 and torch.equal(b, want)
+    one = torch.randn(1, 3, 5, device="cuda")
+    table, lens, refs = torch.full((2, 1), -1, dtype=torch.int32).cuda(), i32(0, 0), i32(0)
+    assert kv_pages.extend(table, lens, refs, i32(1), i32(3), 4).tolist() == [True]
+    assert kv_pages.fork([one], table, lens, refs, i32(1), i32(0), 4).tolist() == [False]   # no second page
+    assert kv_pages.compact([one], table, refs).tolist() == [0] and lens.tolist() == [0, 3]
+
+
+@pytest.mark.parametrize("pages", [4096, 4097, 8192, 9000])
+def test_compaction_at_the_edges_of_its_tiles(built_lib, pages):
+    """Everything in use, nothing in use, all in front, all behind."""
+    cache = torch.arange(pages, dtype=torch.float32, device="cuda").view(pages, 1).repeat(1, 4)
+    for used in (range(0), range(pages), range(pages // 2), range(pages // 2, pages), range(0, pages, 2), range(pages - 1, pages)):
+        refs = torch.zeros(pages, dtype=torch.int32)
+        refs[list(used)] = 1
+        s = oracle.paged.Pages(3, (len(used) + 2) // 3 + 1, pages, 1)
+        s.refs = refs.clone()
+        ids = torch.tensor(list(used), dtype=torch.int32)
+        s.table.view(-1)[:len(used)] = ids[torch.randperm(len(used), generator=torch.Generator().manual_seed(1))]
+        t, r, c = s.table.cuda(), refs.cuda(), cache.clone()
+        before = c[t[t >= 0].long(), 0]
+        mine = c.cpu()
+        page_map = kv_pages.compact([c], t, r)
+        assert torch.equal(page_map.cpu(), s.compact([mine]))
+        assert torch.equal(t.cpu(), s.table) and torch.equal(r.cpu(), s.refs) and torch.equal(c.cpu(), mine)
+        assert torch.equal(c[t[t >= 0].long(), 0], before)
+
+
 @pytest.mark.parametrize("kind", [torch.bfloat16, torch.float8_e4m3fn])
 def test_a_serving_run(built_lib, kind):
     """Prompts come in, one is forked, tokens are added to all, a prompt leaves, the pool is compacted: after every step

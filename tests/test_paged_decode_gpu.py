@@ -268,6 +268,64 @@ def test_two_graphs_of_one_pool(built_lib):
         assert torch.equal(outs[i][0], want[i][0]) and torch.equal(outs[i][1], want[i][1])
 
 
+def test_a_query_that_is_not_aligned(built_lib):
+    a = make([100, 33], 2, 4, 64, BF16, BF16, 16, seed=23)
+    d = on_gpu(a)
+    o, lse = paged_decode.run(**d)
+    flat = torch.zeros(a["q"].numel() + 3, dtype=BF16, device="cuda")
+    flat[3:] = d["q"].flatten()
+    d["q"] = flat[3:].view(a["q"].shape)
+    assert d["q"].data_ptr() % 16 != 0
+    o2, lse2 = paged_decode.run(**d)
+    assert torch.equal(o, o2) and torch.equal(lse, lse2)
+
+
+def test_no_cache_no_table_no_batch(built_lib):
+    q = torch.randn(3, 4, 64, device="cuda").to(BF16)
+    none = torch.zeros(0, 16, 2, 64, dtype=BF16, device="cuda")
+    some = torch.randn(4, 16, 2, 64, device="cuda").to(BF16)
+    table, lens = torch.zeros(3, 2, dtype=torch.int32, device="cuda"), torch.full((3,), 20, dtype=torch.int32, device="cuda")
+    for k, t in ((none, table), (some, table[:, :0]), (none, table[:, :0])):
+        o, lse = paged_decode.run(q, k, k, t, lens, 0.1)
+        assert (o == 0).all() and torch.isinf(lse).all()
+    o, lse = paged_decode.run(q[:0], some, some, table[:0], lens[:0], 0.1)
+    assert o.shape == (0, 4, 64) and lse.shape == (0, 4)
+
+
+def test_many_heads(built_lib):
+    """More pairs of KV heads and query blocks than CTAs are resident."""
+    run_check(make([17, 40], 48, 17, 64, FP16, FP16, 16, seed=24))
+    run_check(make([100], 1, 300, 64, BF16, E4M3, 7, seed=25))
+
+
+def test_two_host_threads_two_streams(built_lib):
+    import threading
+    cases = [make([900, 64, 1200, 0], 2, 4, 128, BF16, kind, 16, seed=26) for kind in (BF16, E4M3)]
+    dev = [on_gpu(a) for a in cases]
+    torch.cuda.synchronize()
+    results, errors = [None, None], []
+
+    def work(i):
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                for _ in range(20):
+                    out = paged_decode.run(**dev[i])
+            s.synchronize()
+            results[i] = out
+        except Exception as e:  # surfaced in the main thread
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for a, out in zip(cases, results):
+        check(a, *out)
+
+
 def test_agrees_with_gqa_decode(built_lib):
     from ako4x_b200 import gqa_decode, workloads as W
     w = W.make_gqa_decode(5, shape_id=7, device="cuda", lens=[300, 1, 17, 2000, 64], extra_pages=9)

@@ -103,6 +103,32 @@ def test_rows_c_status(built_lib):
     assert call(freq=None) == EINVAL
 
 
+def test_norm_c_status(built_lib):
+    L = _cabi.lib()
+    raw = ctypes.create_string_buffer(4096)
+    x = (ctypes.addressof(raw) + 255) & ~255
+    rows = _cabi.HeadRows(x, 128, 64, 2)
+    ref = ctypes.byref
+
+    def call(qw=x, kw=x, out=x, tokens=4):
+        return L.ako4x_qk_norm_rope(ref(rows), ref(rows), qw, kw, 0, 1e-6, x, 0, x, 64, 0, 1.0, x, out, tokens, 64, 0, None)
+
+    assert call(tokens=0) == OK
+    assert call(qw=None) == EINVAL and call(kw=None) == EINVAL and call(out=None) == EINVAL
+    assert call(qw=x + 2) == EINVAL and call(kw=x + 8) == EINVAL
+
+    def store(kc, cdtype=0, slots=x, pages=8, qw=x):
+        return L.ako4x_qk_norm_rope_cache(ref(rows), ref(rows), ref(rows), qw, x, 0, 1e-6, x, 0, x, 64, 0, 1.0, x, slots, 0, ref(kc),
+                                          ref(kc), cdtype, pages, 16, 4, 64, 0, None)
+
+    good = _cabi.KvCache(x, None, 2048, 128, 64, 0, 0, 0)
+    assert store(good, slots=None) == EINVAL and store(good, pages=-1) == EINVAL and store(good, cdtype=1) == ESHAPE
+    assert store(good, qw=x + 2) == EINVAL
+    assert store(_cabi.KvCache(x + 8, None, 2048, 128, 64, 0, 0, 0)) == EINVAL
+    assert store(_cabi.KvCache(x, None, 2048, 132, 66, 0, 0, 0)) == EINVAL
+    assert store(good, cdtype=2) == EINVAL                  # e4m3 without scales
+
+
 def test_frequencies():
     f, m = rope.frequencies(64, base=10000.0, device="cpu")
     i = torch.arange(32, dtype=torch.float64)
@@ -223,6 +249,9 @@ def test_pages_refusals(built_lib):
     _refused(lambda: kv_pages.fork([torch.zeros(7, 4)], table, lens, refs, rows, rows, 16), "first dimension")
     _refused(lambda: kv_pages.compact([torch.zeros(4, 8).T], table, refs), "one piece")
     _refused(lambda: kv_pages.copy([torch.zeros(1, 4).expand(8, 4)], rows, rows), "one piece")
+    _refused(lambda: kv_pages.copy([torch.zeros(8, 3, 4).transpose(1, 2), torch.zeros(8), torch.zeros(8, 0)], rows, rows), "CUDA")
+    _refused(lambda: kv_pages.copy([torch.zeros(8, 3, 4)[:, :, ::2]], rows, rows), "one piece")
+    _refused(lambda: kv_pages.copy([torch.zeros(8, 1, 4).expand(8, 2, 4)], rows, rows), "one piece")
     with pytest.raises(TypeError):
         kv_pages.copy(3, rows, rows)
 

@@ -204,6 +204,35 @@ def test_store_without_norms_and_with_nan(built_lib):
     assert bad[2, 1] and int(bad.sum()) == 1                 # a row with a NaN, and no other, has a scale of NaN
 
 
+def test_weights_and_tables_that_are_views(built_lib):
+    q, k, _ = _qkv(7, 4, 2, 64, BF16, 12)
+    f, _ = rope.frequencies(64)
+    pos = torch.arange(7).cuda()
+    base = (1 + 0.1 * torch.randn(200, generator=torch.Generator().manual_seed(1))).to(BF16).cuda()
+    for w in (base[1:65], base[3:131:2], base.float()[1:65]):
+        a = qk_norm_rope.run(q, k, w, w, pos, f)
+        b = qk_norm_rope.run(q, k, w.clone(), w.clone(), pos, f)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    odd = torch.zeros(33, device="cuda")
+    odd[1:] = f
+    assert torch.equal(rope.run(q, None, pos, odd[1:])[0], rope.run(q, None, pos, f)[0])
+
+
+@pytest.mark.parametrize("tokens", [5919, 5920, 5921, 11843, 23700])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_tokens_side_by_side(built_lib, tokens, interleaved):
+    """Around the sizes at which a warp takes one, two, four and eight tokens; the last warp not full."""
+    for hq, hk, dim, rotary in ((3, 1, 64, 64), (1, 1, 48, 20), (2, 1, 128, 64), (1, 0, 16, 16)):
+        q, k, _ = _qkv(tokens, hq, max(hk, 1), dim, BF16, tokens)
+        k = k[:, :hk]
+        f, _ = rope.frequencies(rotary)
+        pos = _positions(tokens, dim, 100000).cuda()
+        y, z = rope.run(q, k, pos, f, interleaved)
+        for at in range(0, tokens, 3000):                    # pieces too short for that
+            a, b = rope.run(q[at:at + 3000], k[at:at + 3000], pos[at:at + 3000], f, interleaved)
+            assert torch.equal(y[at:at + 3000], a) and torch.equal(z[at:at + 3000], b)
+
+
 def test_captured_and_replayed(built_lib):
     q, k, v = _qkv(20, 8, 2, 128, BF16, 5)
     w = torch.ones(128, dtype=BF16, device="cuda")
