@@ -15,7 +15,8 @@
 // and a lane's second piece holds the partners of its first: nothing is exchanged but the sum of the squares, and
 // nothing is unpacked twice. A warp takes row groups of one token (all of them, or a share where there are few
 // tokens), the loads two groups ahead; the token's R/2 angles are shared out over the lanes once.
-// Interleaved pairs lie in one piece; where R/2 is no multiple of 8 the partners are read again.
+// Interleaved pairs lie in one piece; where R/2 is no multiple of 8 the rotated elements go through shared memory, a pair
+// to a lane.
 // Measured, 8 192 tokens with 32 + 8 + 8 heads of 128 into a bf16 cache (201 MB): one piece per lane and partners by
 // shuffle 72 us; two pieces 61; grid without divisions, tables from whole vectors 51; loads ahead across the kinds of
 // rows, 20 warps to an SM 45 (4.5 TB/s). The same without arithmetic 31: what is left are instructions, 36 for a piece.
@@ -94,12 +95,13 @@ __device__ __forceinline__ float max_nan(float a, float b) {   // a NaN stays
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
 // Where the partner of a rotated element is.
-enum Partner { OTHER_PIECE, SAME_PIECE, MEMORY };
+enum Partner { OTHER_PIECE, SAME_PIECE, STAGED };   // STAGED: anywhere, by way of shared memory
 
 template <class T, int LANES, Partner PARTNER>
-__global__ void __launch_bounds__(WARPS * 32, PARTNER == MEMORY ? 3 : 5) qk_norm_rope_kernel(const Params p) {
+__global__ void __launch_bounds__(WARPS * 32, PARTNER == STAGED ? 4 : 5) qk_norm_rope_kernel(const Params p) {
   constexpr int GROUP = 32 / LANES;   // rows of a warp instruction
   __shared__ __align__(16) float2 s_cs[WARPS][MAX_ANGLES];
+  __shared__ __align__(16) float s_row[PARTNER == STAGED ? WARPS : 1][32 / LANES][PARTNER == STAGED ? LANES * 16 : 1];
   ako::pdl_trigger();
   ako::pdl_wait();   // nothing before this reads what a kernel wrote, and no load below is of the read-only kind
   const int warp = threadIdx.x >> 5, lane32 = threadIdx.x & 31;
@@ -248,28 +250,10 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == MEMORY ? 3 : 5) qk_norm
             B[h][j] = f2(-w[h][2 * j + 1] * cs.y, w[h][2 * j] * cs.y);
           }
         }
-    } else {                          // the partner's weight is met where the partner is read
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float a[2] = {w[h][2 * j], w[h][2 * j + 1]}, b[2] = {0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const int e = (h ? e1 : e0) + 2 * j + c;
-            if (e < p.rotary) {
-              const float2 cs = cs_of[e < half ? e : e - half];
-              a[c] *= cs.x;
-              b[c] = e < half ? -cs.y : cs.y;
-            }
-          }
-          A[h][j] = f2(a[0], a[1]);
-          B[h][j] = f2(b[0], b[1]);
-        }
     }
   };
 
-  const bool all = PARTNER != MEMORY && p.rotary == p.dim;   // every element is rotated
+  const bool all = PARTNER != STAGED && p.rotary == p.dim;   // every element is rotated
   bool ready = false;
 #pragma unroll 1
   for (int it = g0; it < g1;) {       // a kind
@@ -322,7 +306,6 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == MEMORY ? 3 : 5) qk_norm
           const float2 x = Pair<T>::get(word(raw[0][h], j));
           y[h][j] = f2(x.x, x.y);
         }
-      const unsigned char* row = PARTNER == MEMORY ? r.in + token * r.token_stride + min(head, heads - 1) * r.head_stride : nullptr;
       next();
       if (p.ragged) {                 // pieces behind the row's end
 #pragma unroll
@@ -338,24 +321,8 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == MEMORY ? 3 : 5) qk_norm
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            if (PARTNER == OTHER_PIECE) {
-              o[h][j] = y[1 - h][j];
-            } else if (PARTNER == SAME_PIECE) {
-              const float2 x = both(y[h][j]);
-              o[h][j] = f2(x.y, x.x);
-            } else {
-              float v[2];
-#pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                const int e = (h ? e1 : e0) + 2 * j + c, other = e < half ? e + half : e - half;
-                v[c] = 0.f;
-                if (e < p.rotary) {
-                  v[c] = Pair<T>::one(row + other * 2);
-                  if (weight) v[c] *= p.weights32 ? ((const float*)weight)[other] : Pair<T>::one((const T*)weight + other);
-                }
-              }
-              o[h][j] = f2(v[0], v[1]);
-            }
+            if (PARTNER == OTHER_PIECE) o[h][j] = y[1 - h][j];
+            if (PARTNER == SAME_PIECE) o[h][j] = f2(y[h][j].y, y[h][j].x);
           }
         float inv = 1.f;
         if (weight) {
@@ -372,12 +339,38 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == MEMORY ? 3 : 5) qk_norm
           inv = rsqrtf(fmaf(sum, p.inv_dim, p.eps));
         }
         F2 z[2][4];
-        if (all || PARTNER == MEMORY) {   // MEMORY: the partner of an element that is not rotated is 0
+        if (PARTNER == STAGED) {            // a pair to a lane, and back
+          float* staged = s_row[warp][lane32 / LANES];
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              z[h][j] = mul2(y[h][j], A[h][j]);
+              const int e = (h ? e1 : e0) + 2 * j;
+              if (e < p.rotary) *reinterpret_cast<F2*>(staged + e) = z[h][j];
+            }
+          __syncwarp();
+          for (int i = lane; i < half; i += LANES) {
+            const float2 cs = cs_of[i];
+            const float a = staged[i], b = staged[i + half];
+            staged[i] = fmaf(a, cs.x, -b * cs.y);
+            staged[i + half] = fmaf(b, cs.x, a * cs.y);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int e = (h ? e1 : e0) + 2 * j;
+              if (e < p.rotary) z[h][j] = *reinterpret_cast<const F2*>(staged + e);
+            }
+          __syncwarp();                     // read before the next row is put there
+        } else if (all) {
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int j = 0; j < 4; ++j) z[h][j] = fma2(o[h][j], B[h][j], mul2(y[h][j], A[h][j]));
-        } else {                          // an element that is not rotated takes nothing from another one
+        } else {                            // an element that is not rotated takes nothing from another one
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -438,7 +431,7 @@ template <class T, int LANES>
 cudaError_t launch(const Params& p, dim3 blocks, cudaStream_t st) {
   const auto kernel = p.interleaved         ? qk_norm_rope_kernel<T, LANES, SAME_PIECE>
                       : p.rotary % 16 == 0 ? qk_norm_rope_kernel<T, LANES, OTHER_PIECE>
-                                           : qk_norm_rope_kernel<T, LANES, MEMORY>;
+                                           : qk_norm_rope_kernel<T, LANES, STAGED>;
   return ako::launch_pdl(true, kernel, blocks, dim3(WARPS * 32), 0, st, p);
 }
 template <class T>
