@@ -63,7 +63,8 @@ extern "C" int ako4x_paged_decode(const void* q, const ako4x_kv_cache* k_cache, 
     return AKO4X_EINVAL;
   p.same_strides = p.k.page == p.v.page && p.k.slot == p.v.slot;
   const Plan pl = plan_for(batch, q_heads, kv_heads, dim, max_pages, page_size, window, fp8);
-  if (!workspace || workspace_bytes < pl.total) return AKO4X_EWORKSPACE;
+  if (pl.total && (!workspace || workspace_bytes < pl.total)) return AKO4X_EWORKSPACE;
+  if (pl.whole_rows && batch * pl.unit_ctas > 0x7fffffffLL) return AKO4X_ETOOLARGE;
   if ((uintptr_t)workspace & 15) return AKO4X_EINVAL;
   unsigned char* ws = (unsigned char*)workspace;
   p.q = q;
@@ -88,6 +89,7 @@ extern "C" int ako4x_paged_decode(const void* q, const ako4x_kv_cache* k_cache, 
   p.max_pages = (int)max_pages;
   p.window = (int)std::min<int64_t>(window, 0x7fffffff);
   p.shares = pl.shares;
+  p.whole_rows = pl.whole_rows;
   cudaStream_t st = (cudaStream_t)stream;
   return dtype == AKO4X_BF16 ? run_bf16(p, pl, dim, fp8, st) : run_fp16(p, pl, dim, fp8, st);
 }

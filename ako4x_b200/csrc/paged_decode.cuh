@@ -6,27 +6,38 @@
 //
 // in one pass over the keys with the running maximum m, in fp32 from the products on.
 //
-// HBM-bound: a key and its value are read once and met by the few query heads that share them, so nothing is
-// staged: a warp owns one KV head (eight of its query heads) and loads its keys straight into the operand
-// registers of mma.m16n8k16, tokens as M. Lane (g, t) has the 16-byte pieces t + 4 j of tokens g and g + 8;
-// the order of the reduction that this makes is given to q as well. V is loaded the same way and turned by
-// movmatrix, O^T = V^T P^T with features as M. There is no barrier and no shared memory in the loop; the
-// next tile's K is requested when S is computed, its V when O is.
+// HBM-bound: a key and its value are read once and met by the few query heads that share them. A warp owns one KV
+// head (eight of its query heads) and loads its keys straight into the operand registers of mma.m16n8k16, tokens as
+// M: lane (g, t) has the 16-byte pieces t + 4 j of tokens g and g + 8, and the order of the reduction that this makes
+// is given to q as well. V is turned by movmatrix, O^T = V^T P^T with features as M. The loop has no barrier; K of the
+// next tile is requested when S is computed, V of a later one when O is.
+//   * V in registers like K, or, for e4m3 and for 256 features, two tiles of it in shared memory by asynchronous copies that a
+//     lane reads back itself (128 sequences in e4m3: all in registers 235 to 249 us, V in shared memory 218, K too 223;
+//     three of up to 131 072 with 256 features, K and V there: 35, V alone 31).
 //   * P goes in as two pieces of 16 bits, both of them positive for a positive weight, so that an infinite
 //     value stays infinite: hi = P cut to its leading bits, lo = the rest. One piece would put its own rounding
 //     beside the output's, and more of it the fewer keys there are.
+//   * Groups of four query heads and fewer leave half of the eight columns free: the second piece of P goes there, and the
+//     accumulators of the two halves are added at the end (64 sequences of up to 8 192 tokens 166 -> 161 us).
 //   * fp16: P is scaled by 2^15 on its way in (the sum too). A weight of 2^-24 of the largest is the
 //     smallest fp16 value otherwise, and a long tail of keys below it would vanish from o but not from lse.
-//   * Groups of four query heads and fewer leave half of the eight columns free: the second piece of P goes there, and the
-//     accumulators of the two halves are added at the end.
-//   * e4m3 becomes fp16 exactly (one conversion for a pair: 1.6 cycles of an SM for the 128 values of a warp's word,
-//     against 3.6 by shifts to bf16; mma.m16n8k32 on e4m3 itself, with q in pieces, takes more instructions than
-//     that, 113 M against 98 M a call of 128 sequences). The scale of a key multiplies its score. The scale of a value multiplies
-//     its weight, over a power of two above all scales met so far, for fp16's range again.
+//   * e4m3 becomes fp16 exactly, NaN included (one conversion for a pair: 1.6 cycles of an SM for a word of each lane,
+//     against 3.6 by shifts to bf16; mma.m16n8k32 on e4m3 itself, with q in pieces, takes more instructions in all,
+//     113 M against 103 M a call). The scale of a key multiplies its score. The scale of a value multiplies its weight,
+//     over a power of two above all scales met so far, for fp16's range again.
+//   * Pages of whole blocks of 16 tokens need one look-up and one address for a block; others one for every token
+//     (370 -> 300 instructions a block, e4m3 433 -> 390).
 //
-// Work split: flat_share.cuh over tiles of 16 tokens. A CTA's warps take up to four (KV head, block of query heads)
-// pairs; where there are fewer, several warps take a pair's tiles in turn and put their parts together in shared
-// memory. A share that ends inside a sequence leaves a partial (m, l, O) for the merge kernel.
+// Work split: flat_share.cuh over tiles of 16 tokens (32 in e4m3, whose chain from K to O is long). A CTA's warps take
+// up to four (KV head, block of query heads) pairs; where there are fewer, several warps take a pair's tiles in turn
+// and put their parts together in shared memory. A share that ends inside a sequence leaves a partial (m, l, O)
+// for the merge kernel.
+//
+// Measured, whole calls: 64 sequences of up to 8 192 tokens, 32 heads over 8 of 128, bf16 (1.03 GB) 160 to 165 us, 6.3 to
+// 6.5 TB/s, 0.96 to 0.99 of the copy rate. 128 of them in e4m3 (1.19 GB) 209 to 220, 0.83 to 0.87: at full clocks 196 to 215, but this
+// one runs into the power limit (1.6 GHz), and fewer instructions are what helps. Three of up to 131 072 tokens, seven heads over
+// one of 256, fp16 (98 MB) 31, half the rate: five tiles to a warp, which the start, the join and the merge (10) outlast.
+// One of 41 tokens 5.9, 8.1 with shares and merge.
 #pragma once
 #include <algorithm>
 #include <cfloat>
@@ -65,6 +76,7 @@ struct Params {
   int num_pages, page_size, page_shift, max_pages, window;
   int shares;        // CTAs along the tiles
   bool same_strides; // of K and V
+  bool whole_rows;   // a share is one sequence
 };
 
 // Entries for the merge, as in the split of the other decode kernels: {sequence, first share, shares}, one per
@@ -205,12 +217,19 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
   const bool by_share = p.batch > p.shares;
   const bool keeper = unit == 0 && threadIdx.x == 0;
   const bool first_cta = blockIdx.x % p.unit_ctas == 0;
-  const ako::Share sh0 = ako::find_share(p.batch, share, p.shares, s_scan, [&](int r) { return span_of<TILE>(p, r).tiles(); },
+  ako::Share sh0;
+  if (p.whole_rows) {
+    sh0 = {share, 0, span_of<TILE>(p, share).tiles(), 1};
+    if (sh0.left == 0 && first_cta && threadIdx.x < 32)
+      for (int h = lane; h < p.q_heads; h += 32) empty_head<T, D>(p, (int64_t)share * p.q_heads + h);
+  } else {
+    sh0 = ako::find_share(p.batch, share, p.shares, s_scan, [&](int r) { return span_of<TILE>(p, r).tiles(); },
                                          [&](int r) {
                                            if (!first_cta) return;
                                            for (int h = 0; h < p.q_heads; ++h) empty_head<T, D>(p, (int64_t)r * p.q_heads + h);
                                            if (!by_share) p.cut[r] = cut_entry(r, 0, 0);
                                          });
+  }
   int2 cut = cut_entry(0, 0, 0);
   int left = sh0.left, b = sh0.row, skip = sh0.skip;
 
@@ -571,7 +590,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
     }
     const bool whole = te - skip == tiles;
     const int64_t at = by_share ? 2 * (int64_t)share + (skip == 0) : (int64_t)b + share;
-    if (skip == 0) {
+    if (skip == 0 && !p.whole_rows) {
       cut = cut_entry(b, share, whole ? 1 : 1 + (tiles - te + sh0.per - 1) / sh0.per);
       if (!by_share && keeper) p.cut[b] = cut;
     }
@@ -648,7 +667,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
     ++b;
     skip = 0;
   }
-  if (by_share && keeper) p.cut[share] = cut;
+  if (by_share && keeper && !p.whole_rows) p.cut[share] = cut;
 }
 
 // Merge. Few partials of a sequence: a warp per (sequence, head), lanes hold columns.
@@ -779,6 +798,7 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) paged_merge_many_kernel(cons
 struct Plan {
   int head_blocks, per_cta, unit_ctas;
   int shares;
+  bool whole_rows;
   size_t ml, acc, total;   // offsets in the workspace; the entries are first
 };
 inline Plan plan_for(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t max_pages, int64_t page_size, int64_t window,
@@ -794,7 +814,18 @@ inline Plan plan_for(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t d
   int64_t tokens = max_pages * page_size;
   if (window > 0 && tokens > window + TILE) tokens = window + TILE;
   const int64_t tiles = batch * ako::cdiv(tokens, (int64_t)TILE);
-  int64_t shares = std::min(resident / pl.unit_ctas, ako::cdiv(tiles, (int64_t)(WARPS / pl.per_cta)));
+  // Sequences that can only be short (by the table's width, or the window) get a CTA each (for its KV heads), and nothing
+  // is left to merge: up to 4 tiles for a warp, 8 where the CTAs fill the GPU. 32 heads over 8 of 128 in bf16, shares and
+  // merge against this: 1 x 64 tokens 7.4 -> 6.3 us, 20 x 16 5.8 -> 4.0, 200 x 64 13.7 -> 10.3, 200 x 128 21.4 -> 19.2; past
+  // that 1 x 128 7.1 -> 9.5. Eight heads over one: 20 x 16 16.0 -> 4.7.
+  const int64_t along = WARPS / pl.per_cta;
+  pl.whole_rows = ako::cdiv(tokens, TILE) <= (batch * pl.unit_ctas >= resident ? 8 : 4) * along;
+  if (pl.whole_rows) {
+    pl.shares = (int)batch;
+    pl.ml = pl.acc = pl.total = 0;
+    return pl;
+  }
+  int64_t shares = std::min(resident / pl.unit_ctas, ako::cdiv(tiles, along));
   pl.shares = (int)std::max<int64_t>(1, std::min<int64_t>(shares, MERGE_MAX));
   const int64_t entries = std::min<int64_t>(batch, pl.shares), slots = entries + pl.shares;
   pl.ml = (entries * sizeof(int2) + 255) / 256 * 256;
@@ -810,7 +841,7 @@ int launch(const Params& p, const Plan& pl, cudaStream_t st) {
   if (ako::launch_pdl(true, paged_decode_kernel<T, D, FP8, ALIGNED, FOLD>, dim3((unsigned)(pl.shares * pl.unit_ctas)), dim3(THREADS), smem, st, p) !=
       cudaSuccess)
     return AKO4X_ELAUNCH;
-  if (pl.shares == 1) return AKO4X_OK;
+  if (pl.shares == 1 || pl.whole_rows) return AKO4X_OK;
   const int64_t jobs = (int64_t)std::min(p.batch, p.shares) * p.q_heads;
   const bool many = p.shares >= 8LL * p.batch;      // partials of a sequence
   const cudaError_t e = many ? ako::launch_pdl(true, paged_merge_many_kernel<T, D>, dim3((unsigned)jobs * (D / 64)), dim3(MERGE_WARPS * 32), 0, st, p)

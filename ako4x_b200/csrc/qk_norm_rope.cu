@@ -19,7 +19,9 @@
 // to a lane.
 // Measured, 8 192 tokens with 32 + 8 + 8 heads of 128 into a bf16 cache (201 MB): one piece per lane and partners by
 // shuffle 72 us; two pieces 61; grid without divisions, tables from whole vectors 51; loads ahead across the kinds of
-// rows, 20 warps to an SM 45 (4.5 TB/s). The same without arithmetic 31: what is left are instructions, 36 for a piece.
+// rows, 20 warps to an SM 43 to 45 (4.5 to 4.7 TB/s). The same without arithmetic 31: what is left are some 260 instructions
+// for a row group, at half the issue rate. Angles in shared memory for a CTA's tokens instead of tables in registers: 49 to 63; the
+// next row's norm beside this row's rotation: 46; packed fp32 pairs (fma.rn.f32x2): the moves outweigh them.
 #include <algorithm>
 
 #include "common.cuh"

@@ -198,7 +198,7 @@ def test_decode_c_status(built_lib):
     off = _cabi.KvCache(x + 8, None, 4096, 256, 128, 0, 0, 0)
 
     def call(batch=2, hq=4, hk=2, dim=128, pages=8, dtype=0, cdtype=0, k=cache, ws=None, nbytes=0, window=0):
-        return L.ako4x_paged_decode(x, ref(k), ref(cache), x, x, 0.1, window, x, x, batch, hq, hk, dim, pages, 16, 4, dtype, cdtype,
+        return L.ako4x_paged_decode(x, ref(k), ref(cache), x, x, 0.1, window, x, x, batch, hq, hk, dim, pages, 16, 400, dtype, cdtype,
                                     ws, nbytes, None)
 
     assert call(batch=0) == OK
@@ -208,7 +208,7 @@ def test_decode_c_status(built_lib):
     assert call(k=off) == EINVAL
     assert call(cdtype=2) == EINVAL                         # e4m3 without scales
     assert call() == EWORKSPACE and call(ws=x, nbytes=16) == EWORKSPACE
-    need = L.ako4x_paged_decode_workspace_bytes(2, 4, 2, 128, 4, 16, 0)
+    need = L.ako4x_paged_decode_workspace_bytes(2, 4, 2, 128, 400, 16, 0)
     assert need > 0 and call(ws=x + 8, nbytes=need) == EINVAL
     assert L.ako4x_paged_decode_workspace_bytes(2, 5, 2, 128, 4, 16, 0) == 0
 
