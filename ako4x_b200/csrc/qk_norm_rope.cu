@@ -15,8 +15,10 @@
 // and a lane's second piece holds the partners of its first: nothing is exchanged but the sum of the squares, and
 // nothing is unpacked twice. A warp takes row groups of one token (all of them, or a share where there are few
 // tokens), the loads two groups ahead; the token's R/2 angles are shared out over the lanes once.
-// Interleaved pairs lie in one piece; where R/2 is no multiple of 8 the rotated elements go through shared memory, a pair
-// to a lane.
+// Interleaved pairs lie in one piece. Where R/2 is an odd multiple of 4, pieces of 8 bytes and twice the lanes put the
+// partners into one lane; where it is no multiple of 4 the rotated elements go through shared memory, a pair to a lane
+// (8 192 tokens of 40 rows of 64, 40 of them rotated: 60 us so, 18 with the smaller pieces; 5 007 tokens of 96 rows of 80,
+// 40 rotated: 86 and 54. For all sizes the smaller pieces are not better: 48 us for the next paragraph's 45).
 // Measured, 8 192 tokens with 32 + 8 + 8 heads of 128 into a bf16 cache (201 MB): one piece per lane and partners by
 // shuffle 72 us; two pieces 61; grid without divisions, tables from whole vectors 51; loads ahead across the kinds of
 // rows, 20 warps to an SM 43 to 45 (4.5 to 4.7 TB/s). The same without arithmetic 31: what is left are some 260 instructions
@@ -95,15 +97,36 @@ __device__ __forceinline__ float max_nan(float a, float b) {   // a NaN stays
   return r;
 }
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+__device__ __forceinline__ uint32_t word(const uint2& v, int i) { return i == 0 ? v.x : v.y; }
+
+template <int ELEMENTS>   // of two bytes each
+struct Words;
+template <>
+struct Words<8> {
+  using Piece = uint4;
+  static __device__ __forceinline__ void put_once(void* to, const uint32_t (&w)[4]) { __stcs((uint4*)to, make_uint4(w[0], w[1], w[2], w[3])); }
+};
+template <>
+struct Words<4> {
+  using Piece = uint2;
+  static __device__ __forceinline__ void put(void* to, const uint32_t (&w)[2]) { *(uint2*)to = make_uint2(w[0], w[1]); }
+  static __device__ __forceinline__ void put_once(void* to, const uint32_t (&w)[2]) { __stcs((uint2*)to, make_uint2(w[0], w[1])); }
+};
+template <>
+struct Words<2> {
+  static __device__ __forceinline__ void put(void* to, const uint32_t (&w)[1]) { *(uint32_t*)to = w[0]; }
+};
 
 // Where the partner of a rotated element is.
 enum Partner { OTHER_PIECE, SAME_PIECE, STAGED };   // STAGED: anywhere, by way of shared memory
 
-template <class T, int LANES, Partner PARTNER>
-__global__ void __launch_bounds__(WARPS * 32, PARTNER == STAGED ? 4 : 5) qk_norm_rope_kernel(const Params p) {
+// PE: elements of a piece. CTAs to an SM: with the smaller pieces 5, 6, 7 take 64.9, 54.4, 66.4 us for 96 rows of 80.
+template <class T, int LANES, Partner PARTNER, int PE>
+__global__ void __launch_bounds__(WARPS * 32, PARTNER == STAGED ? 4 : PE == 8 ? 5 : 6) qk_norm_rope_kernel(const Params p) {
+  using Piece = typename Words<PE>::Piece;
   constexpr int GROUP = 32 / LANES;   // rows of a warp instruction
   __shared__ __align__(16) float2 s_cs[WARPS][MAX_ANGLES];
-  __shared__ __align__(16) float s_row[PARTNER == STAGED ? WARPS : 1][32 / LANES][PARTNER == STAGED ? LANES * 16 : 1];
+  __shared__ __align__(16) float s_row[PARTNER == STAGED ? WARPS : 1][32 / LANES][PARTNER == STAGED ? LANES * 2 * PE : 1];
   ako::pdl_trigger();
   ako::pdl_wait();   // nothing before this reads what a kernel wrote, and no load below is of the read-only kind
   const int warp = threadIdx.x >> 5, lane32 = threadIdx.x & 31;
@@ -116,9 +139,10 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == STAGED ? 4 : 5) qk_norm
   const int end_q = p.q.groups, end_k = end_q + p.k.groups, end_v = end_k + p.v.groups;
   const int g0 = blockIdx.y * p.per_share, g1 = min(g0 + p.per_share, end_v);
 
-  // this lane's two pieces of a row: the partners of each other in front, neighbours behind
-  const int half = p.rotary / 2, pitch = (half + 1) & ~1, paired = PARTNER == OTHER_PIECE ? p.rotary / 16 : 0;
-  const int e0 = 8 * (lane < paired ? lane : 2 * lane), e1 = 8 * (lane < paired ? lane + paired : 2 * lane + 1);
+  // this lane's two pieces of a row: the partners of each other in front; behind, the lanes' first pieces and then their
+  // second ones, so that an instruction's bytes are one stretch (8 192 tokens of 17 rows of 64, pairs: 11.4 -> 11.0 us)
+  const int half = p.rotary / 2, pitch = (half + 1) & ~1, paired = PARTNER == OTHER_PIECE ? p.rotary / (2 * PE) : 0;
+  const int e0 = PE * (lane < paired ? lane : lane + paired), e1 = PE * (lane < paired ? lane + paired : lane + LANES);
   const bool in0 = e0 < p.dim, in1 = e1 < p.dim;
 
   // The loads run two row groups ahead, from one kind into the next. A lane past the last row, or past the row's
@@ -126,7 +150,7 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == STAGED ? 4 : 5) qk_norm
   int at = g0, at_kind = g0 < end_q ? 0 : g0 < end_k ? 1 : 2, at_stop, at_head, at_heads;
   const unsigned char *from0, *from1;
   int64_t step;
-  uint4 raw[2][2];
+  Piece raw[2][2];
   auto aim = [&] {
     const Rows& r = at_kind == 0 ? p.q : at_kind == 1 ? p.k : p.v;
     const int start = at_kind == 0 ? 0 : at_kind == 1 ? end_q : end_k;
@@ -138,10 +162,10 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == STAGED ? 4 : 5) qk_norm
     from0 += in0 ? e0 * 2 : 0;
     step = slots * r.head_stride;
   };
-  auto fetch = [&](uint4 (&x)[2]) {
+  auto fetch = [&](Piece (&x)[2]) {
     if (at >= g1) return;
-    x[0] = *reinterpret_cast<const uint4*>(from0);
-    x[1] = *reinterpret_cast<const uint4*>(from1);
+    x[0] = *reinterpret_cast<const Piece*>(from0);
+    x[1] = *reinterpret_cast<const Piece*>(from1);
     if (++at == at_stop) {
       if (at < g1) {
         at_kind = at < end_k ? 1 : 2;
@@ -194,26 +218,26 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == STAGED ? 4 : 5) qk_norm
 
   const float2* cs_of = s_cs[warp] + (real ? mine : 0) * pitch;
   // Pairs (2i, 2i + 1) of the pieces' elements: z = inv (x A + x' B), where `mask` says so; inv x A elsewhere.
-  F2 A[2][4], B[2][4];
+  F2 A[2][PE / 2], B[2][PE / 2];
   unsigned mask = 0;
   auto tables = [&](const void* weight) {
-    float w[2][8];
+    float w[2][PE];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int e = h ? e1 : e0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w[h][j] = 1.f;
+      for (int j = 0; j < PE; ++j) w[h][j] = 1.f;
       if (weight && (h ? in1 : in0)) {
         if (p.weights32) {
 #pragma unroll
-          for (int j = 0; j < 8; j += 4) {
+          for (int j = 0; j < PE; j += 4) {
             const float4 y = *reinterpret_cast<const float4*>((const float*)weight + e + j);
             w[h][j] = y.x, w[h][j + 1] = y.y, w[h][j + 2] = y.z, w[h][j + 3] = y.w;
           }
         } else {
-          const uint4 x = *reinterpret_cast<const uint4*>((const T*)weight + e);
+          const Piece x = *reinterpret_cast<const Piece*>((const T*)weight + e);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < PE / 2; ++j) {
             const float2 y = Pair<T>::get(word(x, j));
             w[h][2 * j] = y.x;
             w[h][2 * j + 1] = y.y;
@@ -221,17 +245,17 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == STAGED ? 4 : 5) qk_norm
         }
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < PE / 2; ++j) {
         A[h][j] = f2(w[h][2 * j], w[h][2 * j + 1]);
         B[h][j] = f2(0.f, 0.f);
       }
     }
     mask = 0;
     if (PARTNER == OTHER_PIECE) {
-      if (lane < paired) {            // eight angles, of both pieces
-        mask = 0xffu;
+      if (lane < paired) {            // the angles of both pieces
+        mask = (1u << PE) - 1;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < PE / 2; ++j) {
           const float4 cs = *reinterpret_cast<const float4*>(cs_of + e0 + 2 * j);
           A[0][j] = f2(w[0][2 * j] * cs.x, w[0][2 * j + 1] * cs.z);
           A[1][j] = f2(w[1][2 * j] * cs.x, w[1][2 * j + 1] * cs.z);
@@ -243,11 +267,11 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == STAGED ? 4 : 5) qk_norm
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < PE / 2; ++j) {
           const int e = (h ? e1 : e0) + 2 * j;
           if (e < p.rotary) {
             const float2 cs = cs_of[e / 2];
-            mask |= 1u << (4 * h + j);
+            mask |= 1u << (PE / 2 * h + j);
             A[h][j] = f2(w[h][2 * j] * cs.x, w[h][2 * j + 1] * cs.x);
             B[h][j] = f2(-w[h][2 * j + 1] * cs.y, w[h][2 * j] * cs.y);
           }
@@ -291,20 +315,20 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == STAGED ? 4 : 5) qk_norm
     if (!turn && !quant) {            // values as they are
 #pragma unroll 1
       for (; it < stop; ++it, head += slots, to0 += out_step, to1 += out_step) {
-        const uint4 x0 = raw[0][0], x1 = raw[0][1];
+        const Piece x0 = raw[0][0], x1 = raw[0][1];
         next();
-        if (store && head < heads && in0) __stcs(reinterpret_cast<uint4*>(to0), x0);
-        if (store && head < heads && in1) __stcs(reinterpret_cast<uint4*>(to1), x1);
+        if (store && head < heads && in0) __stcs(reinterpret_cast<Piece*>(to0), x0);
+        if (store && head < heads && in1) __stcs(reinterpret_cast<Piece*>(to1), x1);
       }
     }
 #pragma unroll 1
     for (; it < stop; ++it, head += slots, to0 += out_step, to1 += out_step) {
       const bool live = store && head < heads;
-      F2 y[2][4];
+      F2 y[2][PE / 2];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < PE / 2; ++j) {
           const float2 x = Pair<T>::get(word(raw[0][h], j));
           y[h][j] = f2(x.x, x.y);
         }
@@ -314,15 +338,15 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == STAGED ? 4 : 5) qk_norm
         for (int h = 0; h < 2; ++h)
           if (!(h ? in1 : in0)) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) y[h][j] = f2(0.f, 0.f);
+            for (int j = 0; j < PE / 2; ++j) y[h][j] = f2(0.f, 0.f);
           }
       }
       if (turn) {
-        F2 o[2][4];
+        F2 o[2][PE / 2];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < PE / 2; ++j) {
             if (PARTNER == OTHER_PIECE) o[h][j] = y[1 - h][j];
             if (PARTNER == SAME_PIECE) o[h][j] = f2(y[h][j].y, y[h][j].x);
           }
@@ -330,7 +354,7 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == STAGED ? 4 : 5) qk_norm
         if (weight) {
           F2 ss = mul2(y[0][0], y[0][0]), st = mul2(y[1][0], y[1][0]);
 #pragma unroll
-          for (int j = 1; j < 4; ++j) {
+          for (int j = 1; j < PE / 2; ++j) {
             ss = fma2(y[0][j], y[0][j], ss);
             st = fma2(y[1][j], y[1][j], st);
           }
@@ -340,13 +364,13 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == STAGED ? 4 : 5) qk_norm
           for (int m = LANES / 2; m >= 1; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
           inv = rsqrtf(fmaf(sum, p.inv_dim, p.eps));
         }
-        F2 z[2][4];
+        F2 z[2][PE / 2];
         if (PARTNER == STAGED) {            // a pair to a lane, and back
           float* staged = s_row[warp][lane32 / LANES];
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < PE / 2; ++j) {
               z[h][j] = mul2(y[h][j], A[h][j]);
               const int e = (h ? e1 : e0) + 2 * j;
               if (e < p.rotary) *reinterpret_cast<F2*>(staged + e) = z[h][j];
@@ -362,7 +386,7 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == STAGED ? 4 : 5) qk_norm
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < PE / 2; ++j) {
               const int e = (h ? e1 : e0) + 2 * j;
               if (e < p.rotary) z[h][j] = *reinterpret_cast<const F2*>(staged + e);
             }
@@ -371,21 +395,21 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == STAGED ? 4 : 5) qk_norm
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) z[h][j] = fma2(o[h][j], B[h][j], mul2(y[h][j], A[h][j]));
+            for (int j = 0; j < PE / 2; ++j) z[h][j] = fma2(o[h][j], B[h][j], mul2(y[h][j], A[h][j]));
         } else {                            // an element that is not rotated takes nothing from another one
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < PE / 2; ++j) {
               z[h][j] = mul2(y[h][j], A[h][j]);
-              if (mask >> (4 * h + j) & 1) z[h][j] = fma2(o[h][j], B[h][j], z[h][j]);
+              if (mask >> (PE / 2 * h + j) & 1) z[h][j] = fma2(o[h][j], B[h][j], z[h][j]);
             }
         }
         const F2 by = f2(inv, inv);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) y[h][j] = weight ? mul2(z[h][j], by) : z[h][j];
+          for (int j = 0; j < PE / 2; ++j) y[h][j] = weight ? mul2(z[h][j], by) : z[h][j];
       }
       if (quant) {
         // e4m3 with the row's own scale: amax / 448, 1 for a row of (nearly) zeros
@@ -393,7 +417,7 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == STAGED ? 4 : 5) qk_norm
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < PE / 2; ++j) {
             const float2 x = both(y[h][j]);
             top = max_nan(top, max_nan(fabsf(x.x), fabsf(x.y)));
           }
@@ -402,43 +426,47 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == STAGED ? 4 : 5) qk_norm
         const float sc = top <= 1e-10f ? 1.0f : __fdiv_rn(top, 448.0f);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          uint32_t w[2] = {0u, 0u};
+          uint32_t w[PE / 4] = {};
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < PE / 2; ++j) {
             const float2 x = both(y[h][j]);
             const uint32_t pair = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(x.x, sc), __fdiv_rn(x.y, sc)), __NV_SATFINITE, __NV_E4M3);
             w[j >> 1] |= pair << (16 * (j & 1));
           }
-          if (live && (h ? in1 : in0)) *reinterpret_cast<uint2*>(h ? to1 : to0) = make_uint2(w[0], w[1]);
+          if (live && (h ? in1 : in0)) Words<PE / 2>::put(h ? to1 : to0, w);
         }
         if (live && lane == 0) *scale_out = sc;
         scale_out += scale_step;
       } else {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          uint32_t w[4];
+          uint32_t w[PE / 2];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < PE / 2; ++j) {
             const float2 x = both(y[h][j]);
             w[j] = Pair<T>::put(x.x, x.y);
           }
-          if (live && (h ? in1 : in0)) __stcs(reinterpret_cast<uint4*>(h ? to1 : to0), make_uint4(w[0], w[1], w[2], w[3]));
+          if (live && (h ? in1 : in0)) Words<PE>::put_once(h ? to1 : to0, w);
         }
       }
     }
   }
 }
 
-template <class T, int LANES>
+// Elements of a piece: 8, or 4 where that puts the partners into one lane and 8 does not.
+int piece_of(bool interleaved, int rotary) { return !interleaved && rotary % 16 == 8 ? 4 : 8; }
+
+template <class T, int LANES>   // LANES: of a row, with pieces of 8
 cudaError_t launch(const Params& p, dim3 blocks, cudaStream_t st) {
-  const auto kernel = p.interleaved         ? qk_norm_rope_kernel<T, LANES, SAME_PIECE>
-                      : p.rotary % 16 == 0 ? qk_norm_rope_kernel<T, LANES, OTHER_PIECE>
-                                           : qk_norm_rope_kernel<T, LANES, STAGED>;
+  const auto kernel = p.interleaved         ? qk_norm_rope_kernel<T, LANES, SAME_PIECE, 8>
+                      : p.rotary % 16 == 0 ? qk_norm_rope_kernel<T, LANES, OTHER_PIECE, 8>
+                      : p.rotary % 16 == 8 ? qk_norm_rope_kernel<T, 2 * LANES, OTHER_PIECE, 4>
+                                           : qk_norm_rope_kernel<T, LANES, STAGED, 8>;
   return ako::launch_pdl(true, kernel, blocks, dim3(WARPS * 32), 0, st, p);
 }
 template <class T>
-cudaError_t launch(const Params& p, int lanes, dim3 blocks, cudaStream_t st) {
-  return lanes == 4 ? launch<T, 4>(p, blocks, st) : lanes == 8 ? launch<T, 8>(p, blocks, st) : launch<T, 16>(p, blocks, st);
+cudaError_t launch(const Params& p, dim3 blocks, cudaStream_t st) {
+  return p.dim <= 64 ? launch<T, 4>(p, blocks, st) : p.dim <= 128 ? launch<T, 8>(p, blocks, st) : launch<T, 16>(p, blocks, st);
 }
 
 bool aligned(const void* ptr, int64_t a, int64_t b, int64_t c, int64_t to) {
@@ -450,8 +478,8 @@ int run(Params& p, const ako4x_head_rows* q, const ako4x_head_rows* k, const ako
   if (tokens < 0 || dim < 0 || rotary < 0) return AKO4X_EINVAL;
   if (dim < 8 || dim > MAX_DIM || dim % 8 || rotary > dim || rotary % 2) return AKO4X_EUNSUPPORTED_SHAPE;
   if (dtype != AKO4X_BF16 && dtype != AKO4X_FP16) return AKO4X_EUNSUPPORTED_SHAPE;
-  const int lanes = dim <= 64 ? 4 : dim <= 128 ? 8 : 16;
-  const int group = 32 / lanes;
+  const int padded = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;   // elements of a row with those behind its end
+  const int group = 32 * 2 * piece_of(p.interleaved, (int)rotary) / padded;
   const ako4x_head_rows* in[3] = {q, k, v};
   Rows* to[3] = {&p.q, &p.k, &p.v};
   bool any = false;
@@ -477,7 +505,7 @@ int run(Params& p, const ako4x_head_rows* q, const ako4x_head_rows* k, const ako
   p.dim = (int)dim;
   p.rotary = (int)rotary;
   p.inv_dim = 1.0f / (float)dim;
-  p.ragged = dim != lanes * 16;
+  p.ragged = dim != padded;
   // A warp takes a token's rows; several tokens side by side, as long as there are warps for the GPU, where a token has few
   // (what is done once for a token weighs more then: 8 192 tokens of 17 rows of 64 12.8 -> 11.3 us; with 48 rows of 128
   // 44.7 -> 51.6, the warps are fewer and longer); or a share of the rows while there are fewer warps than the GPU holds.
@@ -497,7 +525,7 @@ int run(Params& p, const ako4x_head_rows* q, const ako4x_head_rows* k, const ako
   if (blocks > 0x7fffffffLL || shares > 65535 || groups > 0x3fffffffLL) return AKO4X_ETOOLARGE;
   const dim3 grid((unsigned)blocks, (unsigned)shares);
   cudaStream_t st = (cudaStream_t)stream;
-  const cudaError_t e = dtype == AKO4X_BF16 ? launch<__nv_bfloat16>(p, lanes, grid, st) : launch<__half>(p, lanes, grid, st);
+  const cudaError_t e = dtype == AKO4X_BF16 ? launch<__nv_bfloat16>(p, grid, st) : launch<__half>(p, grid, st);
   return e == cudaSuccess ? AKO4X_OK : AKO4X_ELAUNCH;
 }
 

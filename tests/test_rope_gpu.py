@@ -40,7 +40,9 @@ def _positions(tokens, seed, far=1 << 20):
 SHAPES = [  # tokens, q heads, k heads, dim, rotary
     (1, 32, 8, 128, 128), (5, 16, 1, 64, 64), (37, 7, 7, 80, 20), (64, 4, 2, 256, 64), (3, 1, 1, 8, 8), (9, 12, 3, 96, 48),
     (2, 5, 1, 192, 96), (130, 3, 1, 72, 72), (11, 2, 1, 104, 2), (700, 40, 8, 128, 64), (6000, 2, 1, 64, 32), (4, 9, 2, 248, 248),
-    (17, 6, 6, 136, 0), (33, 1, 1, 128, 100)]
+    (17, 6, 6, 136, 0), (33, 1, 1, 128, 100),
+    # rotated parts of an odd number of eights: pieces of half the size, in rows of one, two and four to a warp
+    (33, 5, 2, 80, 40), (21, 4, 2, 96, 24), (6000, 2, 1, 64, 40), (13, 3, 1, 256, 200), (1, 1, 0, 24, 24), (10, 2, 2, 64, 26)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP16])
@@ -122,7 +124,8 @@ def test_values_that_are_not_finite_stay_in_their_pairs(built_lib):
         assert torch.equal(torch.isnan(y.cpu()), torch.isnan(ref))
 
 
-CACHES = [(1, 32, 8, 128, 128, 16), (70, 8, 2, 64, 64, 1), (33, 6, 3, 80, 20, 7), (300, 16, 4, 256, 64, 64), (6, 2, 1, 96, 96, 24)]
+CACHES = [(1, 32, 8, 128, 128, 16), (70, 8, 2, 64, 64, 1), (33, 6, 3, 80, 20, 7), (300, 16, 4, 256, 64, 64), (6, 2, 1, 96, 96, 24),
+          (45, 4, 2, 80, 40, 16), (12, 3, 2, 256, 24, 5), (700, 1, 1, 64, 8, 32)]
 
 
 def _cache(pages, ps, hk, dim, kind, layout):
