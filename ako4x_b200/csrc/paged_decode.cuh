@@ -29,15 +29,15 @@
 //     (370 -> 300 instructions a block, e4m3 433 -> 390).
 //
 // Work split: flat_share.cuh over tiles of 16 tokens (32 in e4m3, whose chain from K to O is long). A CTA's warps take
-// up to four (KV head, block of query heads) pairs; where there are fewer, several warps take a pair's tiles in turn
-// and put their parts together in shared memory. A share that ends inside a sequence leaves a partial (m, l, O)
+// up to four (KV head, block of query heads) pairs; where there are fewer, or short sequences that fit the GPU at once,
+// several warps take a pair's tiles in turn and put their parts together in shared memory. A share that ends inside a sequence leaves a partial (m, l, O)
 // for the merge kernel.
 //
 // Measured, whole calls: 64 sequences of up to 8 192 tokens, 32 heads over 8 of 128, bf16 (1.03 GB) 160 to 165 us, 6.3 to
 // 6.5 TB/s, 0.96 to 0.99 of the copy rate. 128 of them in e4m3 (1.19 GB) 209 to 220, 0.83 to 0.87: at full clocks 196 to 215, but this
 // one runs into the power limit (1.6 GHz), and fewer instructions are what helps. Three of up to 131 072 tokens, seven heads over
 // one of 256, fp16 (98 MB) 31, half the rate: five tiles to a warp, which the start, the join and the merge (10) outlast.
-// One of 41 tokens 5.9, 8.1 with shares and merge.
+// One of 41 tokens 5.3, 5.9 with a warp to a pair, 8.1 with shares and merge.
 #pragma once
 #include <algorithm>
 #include <cfloat>
@@ -813,13 +813,21 @@ inline Plan plan_for(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t d
   const int64_t TILE = BLOCK * blocks(dim, fp8);
   int64_t tokens = max_pages * page_size;
   if (window > 0 && tokens > window + TILE) tokens = window + TILE;
-  const int64_t tiles = batch * ako::cdiv(tokens, (int64_t)TILE);
+  const int64_t each = ako::cdiv(tokens, TILE), tiles = batch * each;
   // Sequences that can only be short (by the table's width, or the window) get a CTA each (for its KV heads), and nothing
-  // is left to merge: up to 4 tiles for a warp, 8 where the CTAs fill the GPU. 32 heads over 8 of 128 in bf16, shares and
+  // is left to merge: up to 4 tiles for a warp, 8 where there are CTAs enough. 32 heads over 8 of 128 in bf16, shares and
   // merge against this: 1 x 64 tokens 7.4 -> 6.3 us, 20 x 16 5.8 -> 4.0, 200 x 64 13.7 -> 10.3, 200 x 128 21.4 -> 19.2; past
   // that 1 x 128 7.1 -> 9.5. Eight heads over one: 20 x 16 16.0 -> 4.7.
+  // While the GPU holds a CTA for every pair, the four warps of a CTA share one pair's tiles: 1 x 64 tokens 6.3 -> 4.2 us,
+  // 1 x 128 7.2 -> 5.0, 40 x 256 14.6 -> 10.0; with twice the pairs 60 x 64 8.2 -> 8.9 and 120 x 64 9.1 -> 13.6. 512 tokens, 8 tiles
+  // for a warp: 24 x 8 pairs 18.9 -> 15.4, 8 x 8 10.9 -> 10.5, but 1 x 8 7.5 -> 10.1 and 24 x 1 9.9 -> 11.8.
+  const bool spread = batch * units <= resident && each > 1 && each <= (8 * batch * units >= resident ? 8 : 4) * WARPS;
+  if (spread) {
+    pl.per_cta = 1;
+    pl.unit_ctas = (int)units;
+  }
   const int64_t along = WARPS / pl.per_cta;
-  pl.whole_rows = ako::cdiv(tokens, TILE) <= (batch * pl.unit_ctas >= resident ? 8 : 4) * along;
+  pl.whole_rows = spread || each <= (batch * pl.unit_ctas >= resident ? 8 : 4) * along;
   if (pl.whole_rows) {
     pl.shares = (int)batch;
     pl.ml = pl.acc = pl.total = 0;

@@ -75,6 +75,16 @@ def test_heads_sizes_types(built_lib, hk, group, dim, dtype, kind):
 
 
 @pytest.mark.parametrize("dtype,kind", TYPES)
+@pytest.mark.parametrize("hk,group,dim", [(8, 4, 128), (4, 9, 64), (2, 5, 256)])
+@pytest.mark.parametrize("batch,longest,window", [(1, 31, 0), (9, 65, 0), (130, 65, 0), (1, 255, 0), (30, 257, 0), (9, 512, 0), (1, 513, 0),
+                                                  (24, 300, 130), (1, 700, 130)])
+def test_short_tables_of_several_heads(built_lib, batch, longest, window, hk, group, dim, dtype, kind):
+    """The warps of a CTA share a pair's tiles, take a pair each, or split the batch into shares, by what the table can hold."""
+    lens = [longest - (i * 37) % (longest + 1) for i in range(batch)]
+    run_check(make(lens, hk, group, dim, dtype, kind, 16 if batch % 2 else 5, seed=longest + batch), **({"window": window} if window else {}))
+
+
+@pytest.mark.parametrize("dtype,kind", TYPES)
 @pytest.mark.parametrize("ps", [1, 2, 7, 16, 24, 64, 100])
 def test_page_sizes_end_inside_a_tile(built_lib, ps, dtype, kind):
     run_check(make([1, ps, ps + 1, 3 * ps - 1, 200, 16, 15], 2, 4, 128, dtype, kind, ps, seed=ps))
