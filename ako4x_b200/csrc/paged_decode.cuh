@@ -22,9 +22,10 @@
 //   * fp16: P is scaled by 2^15 on its way in (the sum too). A weight of 2^-24 of the largest is the
 //     smallest fp16 value otherwise, and a long tail of keys below it would vanish from o but not from lse.
 //   * e4m3 becomes fp16 exactly, NaN included (one conversion for a pair: 1.6 cycles of an SM for a word of each lane,
-//     against 3.6 by shifts to bf16; mma.m16n8k32 on e4m3 itself, with q in pieces, takes more instructions in all,
-//     113 M against 103 M a call). The scale of a key multiplies its score. The scale of a value multiplies its weight,
-//     over a power of two above all scales met so far, for fp16's range again.
+//     against 3.6 by shifts to bf16; mma.m16n8k32 on e4m3 itself, with q in pieces, takes more instructions in all), and V
+//     goes on to bf16, exact too. The scale of a key multiplies its score, the scale of a value its weight: these products differ by as much
+//     as scales do (a row of zeros is stored with the scale 1), and need the exponents. On tf32 the same is slower: 64
+//     sequences with seven heads over each of four 64 against 61 us.
 //   * Pages of whole blocks of 16 tokens need one look-up and one address for a block; others one for every token
 //     (370 -> 300 instructions a block, e4m3 433 -> 390).
 //
@@ -137,14 +138,13 @@ __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e 
 // e with 2^e <= x < 2^(e + 1), within [-120, 120]
 __device__ __forceinline__ int exponent(float x) { return min(max(((int)(__float_as_uint(x) >> 23) & 0xff) - 127, -120), 120); }
 
-// A weight p >= 0 as hi + lo, both positive where p is.
+// A weight p >= 0 as hi + lo, both positive where p is: in bf16 p cut to its leading bits, and the rest with 2^-20 of p.
 template <class T>
 __device__ __forceinline__ void two_pieces(float p0, float p1, uint32_t& hi, uint32_t& lo);
 template <>
 __device__ __forceinline__ void two_pieces<__nv_bfloat16>(float p0, float p1, uint32_t& hi, uint32_t& lo) {
-  hi = __byte_perm(__float_as_uint(p0), __float_as_uint(p1), 0x7632);   // cut
-  const float r0 = p0 - ako::bf16_lo(hi), r1 = p1 - ako::bf16_hi(hi);
-  lo = ako::pack_bf16x2(r0 == 0.f ? p0 * 0x1p-16f : r0, r1 == 0.f ? p1 * 0x1p-16f : r1);
+  hi = __byte_perm(__float_as_uint(p0), __float_as_uint(p1), 0x7632);
+  lo = ako::pack_bf16x2(fmaf(p0, 1.f + 0x1p-20f, -ako::bf16_lo(hi)), fmaf(p1, 1.f + 0x1p-20f, -ako::bf16_hi(hi)));
 }
 template <>
 __device__ __forceinline__ void two_pieces<__half>(float p0, float p1, uint32_t& hi, uint32_t& lo) {
@@ -155,14 +155,7 @@ __device__ __forceinline__ void two_pieces<__half>(float p0, float p1, uint32_t&
   __half2 l = __floats2half2_rn(r0, r1);
   lo = *reinterpret_cast<uint32_t*>(&l);
 }
-// The same where no value is infinite: any weight, rounded, and the rest.
-__device__ __forceinline__ void two_rounded(float p0, float p1, uint32_t& hi, uint32_t& lo) {
-  __half2 h = __floats2half2_rn(p0, p1);
-  hi = *reinterpret_cast<uint32_t*>(&h);
-  const float2 c = __half22float2(h);
-  __half2 l = __floats2half2_rn(p0 - c.x, p1 - c.y);
-  lo = *reinterpret_cast<uint32_t*>(&l);
-}
+__device__ __forceinline__ float2 unpack_half(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
 
 template <class T>
 __device__ __forceinline__ uint32_t pack2(float a, float b);
@@ -201,8 +194,9 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
   constexpr bool RINGED = ringed(D, FP8);
   constexpr int TT = blocks(D, FP8), TILE = BLOCK * TT, R = 2 * TT;   // R: tokens of a lane in a tile
   constexpr int SLOT = R * NJ * 512, PART = warp_bytes(D, FP8);      // V of a tile; what a warp has of shared memory
-  using TM = typename std::conditional<FP8, __half, T>::type;   // operand type
-  constexpr float LIFT = std::is_same<TM, __half>::value ? 15.f : 0.f;
+  using TM = typename std::conditional<FP8, __half, T>::type;   // operand type of Q K^T
+  using TV = typename std::conditional<FP8, __nv_bfloat16, T>::type;   // and of P V
+  constexpr float LIFT = std::is_same<TV, __half>::value ? 15.f : 0.f;
   __shared__ int s_scan[6];
   extern __shared__ __align__(16) unsigned char s_ring[];   // [warp]: its tiles, and then its part
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -368,9 +362,6 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
       qs0 *= __shfl_sync(0xffffffffu, back, 8 * t);
       qs1 *= __shfl_sync(0xffffffffu, back, 8 * t + 4);
     }
-    // e4m3: the weights of P times their scales, over 2^unit > all scales met so far, are what goes into the product
-    int unit_v = -121;
-    float over = 0.f, under = 0.f;                  // 2^unit, 2^-unit
     // acc[i]: rows g and g + 8 of O^T step i, heads 2t and 2t + 1
     float acc[KS][4];
 #pragma unroll
@@ -499,30 +490,9 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
             }
       }
       if (FP8) {
-        float top = 0.f;
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-          vs[i] = now[i] ? vs[i] : 0.f;
-          top = fmaxf(top, fabsf(vs[i]));
-        }
-        if (__any_sync(0xffffffffu, top >= over)) {
-#pragma unroll
-          for (int o = 4; o <= 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          const int u = max(unit_v, exponent(top) + 1);
-          if (u != unit_v) {
-            const float f = unit_v == -121 ? 0.f : power_of_two(max(unit_v - u, -126));
-#pragma unroll
-            for (int i = 0; i < KS; ++i)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) acc[i][j] *= f;
-            unit_v = u;
-            over = power_of_two(u);
-            under = power_of_two(-u);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-          const float f = vs[i] * under;
+          const float f = now[i] ? vs[i] : 0.f;
           e[i][0] *= f;
           e[i][1] *= f;
         }
@@ -530,8 +500,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
       uint32_t bh[R], bl[R];
 #pragma unroll
       for (int i = 0; i < R; ++i) {
-        if (FP8) two_rounded(e[i][0], e[i][1], bh[i], bl[i]);
-        else two_pieces<TM>(e[i][0], e[i][1], bh[i], bl[i]);
+        two_pieces<TV>(e[i][0], e[i][1], bh[i], bl[i]);
         if (FOLD) {
           bh[i] = ako::movmatrix_trans(t < 2 ? bh[i] : bl[i]);
         } else {
@@ -547,17 +516,24 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
           const uint4 y = RINGED ? lds16(at_slot + ((2 * u + 1) * NJ + j) * 512) : vc[RINGED ? 0 : 2 * u + 1][RINGED ? 0 : j];
 #pragma unroll
           for (int i = 0; i < (FP8 ? 4 : 2); ++i) {
-            uint32_t x0, x1, y0, y1;
-            if (FP8) {
-              widen(word(x, i), x0, x1);
-              widen(word(y, i), y0, y1);
-            } else {
-              x0 = word(x, 2 * i), x1 = word(x, 2 * i + 1), y0 = word(y, 2 * i), y1 = word(y, 2 * i + 1);
-            }
-            const uint32_t a[4] = {ako::movmatrix_trans(x0), ako::movmatrix_trans(x1), ako::movmatrix_trans(y0), ako::movmatrix_trans(y1)};
             float(&d)[4] = acc[(FP8 ? 4 : 2) * j + i];
-            if (!FOLD) mma<TM>(d, a, bl[2 * u], bl[2 * u + 1]);
-            mma<TM>(d, a, bh[2 * u], bh[2 * u + 1]);
+            uint32_t a[4];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const uint4& z = c ? y : x;
+              if (FP8) {                           // turned in pairs of features: (f, f + 1) of token 2t, then of token 2t + 1
+                uint32_t w0, w1;
+                widen(ako::movmatrix_trans(word(z, i)), w0, w1);
+                const float2 v0 = unpack_half(w0), v1 = unpack_half(w1);
+                a[2 * c] = ako::pack_bf16x2(v0.x, v1.x);
+                a[2 * c + 1] = ako::pack_bf16x2(v0.y, v1.y);
+              } else {
+                a[2 * c] = ako::movmatrix_trans(word(z, 2 * i));
+                a[2 * c + 1] = ako::movmatrix_trans(word(z, 2 * i + 1));
+              }
+            }
+            if (!FOLD) mma<TV>(d, a, bl[2 * u], bl[2 * u + 1]);
+            mma<TV>(d, a, bh[2 * u], bh[2 * u + 1]);
           }
         }
       if (RINGED) {
@@ -579,14 +555,11 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
       l1 += __shfl_xor_sync(0xffffffffu, l1, o);
     }
 
-    if (FP8 || FOLD) {
+    if (FOLD) {
 #pragma unroll
       for (int i = 0; i < KS; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (FOLD) acc[i][j] += __shfl_xor_sync(0xffffffffu, acc[i][j], 2);   // both pieces of P
-          if (FP8) acc[i][j] *= over;
-        }
+        for (int j = 0; j < 4; ++j) acc[i][j] += __shfl_xor_sync(0xffffffffu, acc[i][j], 2);   // both pieces of P
     }
     const bool whole = te - skip == tiles;
     const int64_t at = by_share ? 2 * (int64_t)share + (skip == 0) : (int64_t)b + share;
@@ -594,8 +567,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
       cut = cut_entry(b, share, whole ? 1 : 1 + (tiles - te + sh0.per - 1) / sh0.per);
       if (!by_share && keeper) p.cut[b] = cut;
     }
-    // Lanes g = 2 x and 2 x + 1 hold the even and the odd of eight neighbouring features (16 bits) or of four and the next
-    // four (e4m3): swap, so that the even lane has the first four and the odd one the last four.
+    // Lanes g = 2 x and 2 x + 1 hold the even and the odd of eight neighbouring features (16 bits), or every other pair of
+    // four and the next four (e4m3): swap, so that the even lane has the first four and the odd one the last four.
     const bool odd = g & 1;
     auto each_four = [&](auto&& put) {             // put(head of the block, feature, four values)
 #pragma unroll
@@ -605,7 +578,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
           const float a = acc[i][hh], c = acc[i][2 + hh], e = acc[i + 1][hh], f = acc[i + 1][2 + hh];
           const float r0 = __shfl_xor_sync(0xffffffffu, odd ? a : e, 4), r1 = __shfl_xor_sync(0xffffffffu, odd ? c : f, 4);
           const int col = FP8 ? 64 * (i / 4) + 16 * (g >> 1) + 4 * (i % 4) : 32 * (i / 2) + 8 * (g >> 1);
-          put(2 * t + hh, col + 4 * (g & 1), odd ? make_float4(r0, e, r1, f) : make_float4(a, r0, c, r1));
+          put(2 * t + hh, col + 4 * (g & 1), FP8 ? odd ? make_float4(r0, r1, e, f) : make_float4(a, c, r0, r1)
+                                                 : odd ? make_float4(r0, e, r1, f) : make_float4(a, r0, c, r1));
         }
     };
     auto finish = [&](int h, int col, float4 x, float inv) {
