@@ -14,13 +14,14 @@
 //   * V in registers like K, or, for e4m3 and for 256 features, two tiles of it in shared memory by asynchronous copies that a
 //     lane reads back itself (128 sequences in e4m3: all in registers 235 to 249 us, V in shared memory 218, K too 223;
 //     three of up to 131 072 with 256 features, K and V there: 35, V alone 31).
-//   * P goes in as two pieces of 16 bits, both of them positive for a positive weight, so that an infinite
-//     value stays infinite: hi = P cut to its leading bits, lo = the rest. One piece would put its own rounding
-//     beside the output's, and more of it the fewer keys there are.
+//   * P goes in as two pieces of bf16, which have the exponents of fp32, so that a weight counts however small it is beside
+//     the others; both are positive for a positive weight, so that an infinite value stays infinite: hi = P cut to its leading bits,
+//     lo = the rest. One piece would put its own rounding beside the output's, and more of it the fewer keys there are.
 //   * Groups of four query heads and fewer leave half of the eight columns free: the second piece of P goes there, and the
 //     accumulators of the two halves are added at the end (64 sequences of up to 8 192 tokens 166 -> 161 us).
-//   * fp16: P is scaled by 2^15 on its way in (the sum too). A weight of 2^-24 of the largest is the
-//     smallest fp16 value otherwise, and a long tail of keys below it would vanish from o but not from lse.
+//   * fp16: P V on tf32 (mma.m16n8k8), which holds P's pieces and fp16 values exactly. Two pieces of P in fp16 end at 2^-39
+//     of the largest weight, and where the key that has it has no value, what lies below is all there is. (64 sequences of up to
+//     8 192 tokens 156 us both ways, 28 heads over 4 84 in fp16, 87 on tf32.)
 //   * e4m3 becomes fp16 exactly, NaN included (one conversion for a pair: 1.6 cycles of an SM for a word of each lane,
 //     against 3.6 by shifts to bf16; mma.m16n8k32 on e4m3 itself, with q in pieces, takes more instructions in all), and V
 //     goes on to bf16, exact too. The scale of a key multiplies its score, the scale of a value its weight: these products differ by as much
@@ -138,22 +139,17 @@ __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e 
 // e with 2^e <= x < 2^(e + 1), within [-120, 120]
 __device__ __forceinline__ int exponent(float x) { return min(max(((int)(__float_as_uint(x) >> 23) & 0xff) - 127, -120), 120); }
 
-// A weight p >= 0 as hi + lo, both positive where p is: in bf16 p cut to its leading bits, and the rest with 2^-20 of p.
-template <class T>
-__device__ __forceinline__ void two_pieces(float p0, float p1, uint32_t& hi, uint32_t& lo);
-template <>
-__device__ __forceinline__ void two_pieces<__nv_bfloat16>(float p0, float p1, uint32_t& hi, uint32_t& lo) {
+// A weight p >= 0 as hi + lo, both positive where p is: p cut to its leading bits, and the rest with 2^-20 of p.
+__device__ __forceinline__ void two_pieces(float p0, float p1, uint32_t& hi, uint32_t& lo) {
   hi = __byte_perm(__float_as_uint(p0), __float_as_uint(p1), 0x7632);
   lo = ako::pack_bf16x2(fmaf(p0, 1.f + 0x1p-20f, -ako::bf16_lo(hi)), fmaf(p1, 1.f + 0x1p-20f, -ako::bf16_hi(hi)));
 }
-template <>
-__device__ __forceinline__ void two_pieces<__half>(float p0, float p1, uint32_t& hi, uint32_t& lo) {
-  __half2 h = __halves2half2(__float2half_rz(p0), __float2half_rz(p1));
-  hi = *reinterpret_cast<uint32_t*>(&h);
-  const float2 c = __half22float2(h);
-  const float r0 = p0 > 0.f ? fmaxf(p0 - c.x, 0x1p-24f) : p0, r1 = p1 > 0.f ? fmaxf(p1 - c.y, 0x1p-24f) : p1;
-  __half2 l = __floats2half2_rn(r0, r1);
-  lo = *reinterpret_cast<uint32_t*>(&l);
+// D (16 x 8) += A (16 x 8, row) B (8 x 8, column), both with eight bits of exponent and ten behind the point.
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const float (&a)[4], float b0, float b1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(__float_as_uint(a[0])), "r"(__float_as_uint(a[1])), "r"(__float_as_uint(a[2])), "r"(__float_as_uint(a[3])),
+        "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
 }
 __device__ __forceinline__ float2 unpack_half(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
 
@@ -195,8 +191,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
   constexpr int TT = blocks(D, FP8), TILE = BLOCK * TT, R = 2 * TT;   // R: tokens of a lane in a tile
   constexpr int SLOT = R * NJ * 512, PART = warp_bytes(D, FP8);      // V of a tile; what a warp has of shared memory
   using TM = typename std::conditional<FP8, __half, T>::type;   // operand type of Q K^T
-  using TV = typename std::conditional<FP8, __nv_bfloat16, T>::type;   // and of P V
-  constexpr float LIFT = std::is_same<TV, __half>::value ? 15.f : 0.f;
+  constexpr bool WIDE = !FP8 && std::is_same<T, __half>::value;  // P V on tf32, otherwise on bf16
   __shared__ int s_scan[6];
   extern __shared__ __align__(16) unsigned char s_ring[];   // [warp]: its tiles, and then its part
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -473,8 +468,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
       }
 #pragma unroll
       for (int i = 0; i < R; ++i) {
-        e[i][0] = ako::fast_exp2(e[i][0] - m0 + LIFT);
-        e[i][1] = ako::fast_exp2(e[i][1] - m1 + LIFT);
+        e[i][0] = ako::fast_exp2(e[i][0] - m0);
+        e[i][1] = ako::fast_exp2(e[i][1] - m1);
         l0 += e[i][0];
         l1 += e[i][1];
       }
@@ -500,7 +495,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
       uint32_t bh[R], bl[R];
 #pragma unroll
       for (int i = 0; i < R; ++i) {
-        two_pieces<TV>(e[i][0], e[i][1], bh[i], bl[i]);
+        two_pieces(e[i][0], e[i][1], bh[i], bl[i]);
         if (FOLD) {
           bh[i] = ako::movmatrix_trans(t < 2 ? bh[i] : bl[i]);
         } else {
@@ -517,23 +512,34 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
 #pragma unroll
           for (int i = 0; i < (FP8 ? 4 : 2); ++i) {
             float(&d)[4] = acc[(FP8 ? 4 : 2) * j + i];
-            uint32_t a[4];
+            if (WIDE) {                              // eight tokens at a time: as k = t and t + 4 the tokens 2t and 2t + 1
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const uint4& z = c ? y : x;
-              if (FP8) {                           // turned in pairs of features: (f, f + 1) of token 2t, then of token 2t + 1
-                uint32_t w0, w1;
-                widen(ako::movmatrix_trans(word(z, i)), w0, w1);
-                const float2 v0 = unpack_half(w0), v1 = unpack_half(w1);
-                a[2 * c] = ako::pack_bf16x2(v0.x, v1.x);
-                a[2 * c + 1] = ako::pack_bf16x2(v0.y, v1.y);
-              } else {
-                a[2 * c] = ako::movmatrix_trans(word(z, 2 * i));
-                a[2 * c + 1] = ako::movmatrix_trans(word(z, 2 * i + 1));
+              for (int c = 0; c < 2; ++c) {
+                const uint4& z = c ? y : x;
+                const float2 v0 = unpack_half(ako::movmatrix_trans(word(z, 2 * i))), v1 = unpack_half(ako::movmatrix_trans(word(z, 2 * i + 1)));
+                const float a[4] = {v0.x, v1.x, v0.y, v1.y};
+                if (!FOLD) mma_tf32(d, a, ako::bf16_lo(bl[2 * u + c]), ako::bf16_hi(bl[2 * u + c]));
+                mma_tf32(d, a, ako::bf16_lo(bh[2 * u + c]), ako::bf16_hi(bh[2 * u + c]));
               }
+            } else {
+              uint32_t a[4];
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                const uint4& z = c ? y : x;
+                if (FP8) {                           // turned in pairs of features: (f, f + 1) of token 2t, then of token 2t + 1
+                  uint32_t w0, w1;
+                  widen(ako::movmatrix_trans(word(z, i)), w0, w1);
+                  const float2 v0 = unpack_half(w0), v1 = unpack_half(w1);
+                  a[2 * c] = ako::pack_bf16x2(v0.x, v1.x);
+                  a[2 * c + 1] = ako::pack_bf16x2(v0.y, v1.y);
+                } else {
+                  a[2 * c] = ako::movmatrix_trans(word(z, 2 * i));
+                  a[2 * c + 1] = ako::movmatrix_trans(word(z, 2 * i + 1));
+                }
+              }
+              if (!FOLD) ako::mma_bf16_16816(d, a, bl[2 * u], bl[2 * u + 1]);
+              ako::mma_bf16_16816(d, a, bh[2 * u], bh[2 * u + 1]);
             }
-            if (!FOLD) mma<TV>(d, a, bl[2 * u], bl[2 * u + 1]);
-            mma<TV>(d, a, bh[2 * u], bh[2 * u + 1]);
           }
         }
       if (RINGED) {
@@ -594,8 +600,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
     auto finish_ml = [&](int h, float m, float l) {
       if (h >= heads) return;
       const int64_t head = head0 + h;
-      if (whole) p.lse[(int64_t)b * p.q_heads + head] = l == 0.f ? -INFINITY : (m - LIFT) + log2f(l);
-      else *reinterpret_cast<float2*>(p.part_ml + (at * p.q_heads + head) * 2) = make_float2(m - LIFT, l);
+      if (whole) p.lse[(int64_t)b * p.q_heads + head] = l == 0.f ? -INFINITY : m + log2f(l);
+      else *reinterpret_cast<float2*>(p.part_ml + (at * p.q_heads + head) * 2) = make_float2(m, l);
     };
     if (along == 1) {
       const float i0 = l0 == 0.f ? 0.f : 1.f / l0, i1 = l1 == 0.f ? 0.f : 1.f / l1;

@@ -111,3 +111,43 @@ def test_values_near_the_end_of_bf16(built_lib, lens, hk, group, dim, ps):
     a = make([min(n, 700) for n in lens], hk, group, dim, BF16, E4M3, ps, seed=dim + 3)
     a["v_scale"] = a["v_scale"] * 50 * 2.0 ** 107
     run_check(a)
+
+
+# ---- 16-bit caches ------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("nats", [16, 24, 27, 29, 33])
+@pytest.mark.parametrize("lens,hk,group,dim,ps", LAYOUTS)
+def test_a_key_without_a_value_far_above_the_others(built_lib, lens, hk, group, dim, ps, nats, dtype):
+    """One key takes all the weight, its value is zero, and the others have the largest values that the type holds."""
+    a = make(lens, hk, group, dim, dtype, dtype, ps, seed=dim + nats)
+    a["q"] = a["q"].abs()
+    big = 60000.0 if dtype == FP16 else 1e30
+    a["v_cache"] = (a["v_cache"].float().sign() * big).to(dtype)
+    a["v_cache"][..., ::2] = big                             # no signs that cancel in every other feature
+    mean = a["q"].float().mean() * dim ** 0.5                # of a score with ones
+    for b, n in enumerate(lens):
+        where = at(a, b, n - 1)
+        a["v_cache"][where], a["k_cache"][where] = 0, float(nats / mean)
+    run_check(a)
+
+
+@pytest.mark.parametrize("dtype,kind", [(BF16, BF16), (FP16, FP16)])
+@pytest.mark.parametrize("nats", [20, 30, 45, 60])
+@pytest.mark.parametrize("lens,hk,group,dim,ps", LAYOUTS)
+def test_an_infinite_value_far_below_the_others(built_lib, lens, hk, group, dim, ps, nats, dtype, kind):
+    """It counts, however little its key weighs."""
+    a = make(lens, hk, group, dim, dtype, kind, ps, seed=dim + nats)
+    a["q"] = a["q"].abs()
+    a["k_cache"] = (a["k_cache"].float() * 0.25).to(kind)
+    mean = a["q"].float().mean() * dim ** 0.5
+    for b, n in enumerate(lens):
+        where = at(a, b, n // 2)
+        a["k_cache"][where] = -float(nats / mean)
+        a["v_cache"][where][..., 3], a["v_cache"][where][..., 8] = float("inf"), float("-inf")
+    o, lse = paged_decode.run(**on_gpu(a))
+    ro, rlse, *_ = oracle.paged.paged_decode(**a)
+    assert (ro[..., 3] == float("inf")).all() and (ro[..., 8] == float("-inf")).all()
+    o = o.cpu().double()
+    assert torch.equal(o[..., 3], ro[..., 3]) and torch.equal(o[..., 8], ro[..., 8])
+    assert int(torch.isfinite(o).sum()) == o.numel() // dim * (dim - 2)
