@@ -791,8 +791,8 @@ inline Plan plan_for(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t d
   // All CTAs resident at once, and a tile at least for a warp. What the lengths are is known on the device only.
   const int64_t resident = (int64_t)ako::sm_count() * ctas_per_sm(dim, fp8);
   const int64_t TILE = BLOCK * blocks(dim, fp8);
-  int64_t tokens = max_pages * page_size;
-  if (window > 0 && tokens > window + TILE) tokens = window + TILE;
+  int64_t tokens = std::min<int64_t>(max_pages * page_size, 0x7fffff00);   // more are not read
+  if (window > 0 && tokens - TILE > window) tokens = window + TILE;
   const int64_t each = ako::cdiv(tokens, TILE), tiles = batch * each;
   // Sequences that can only be short (by the table's width, or the window) get a CTA each (for its KV heads), and nothing
   // is left to merge: up to 4 tiles for a warp, 8 where there are CTAs enough. 32 heads over 8 of 128 in bf16, shares and

@@ -213,6 +213,18 @@ def test_decode_c_status(built_lib):
     assert L.ako4x_paged_decode_workspace_bytes(2, 5, 2, 128, 4, 16, 0) == 0
 
 
+def test_decode_plans_of_any_window(built_lib):
+    """A window that no sequence reaches plans like none; a table of more tokens than are read like one of those."""
+    L = _cabi.lib()
+    need = lambda pages, ps, window, batch=1: L.ako4x_paged_decode_workspace_bytes(batch, 32, 8, 128, pages, ps, window)  # noqa: E731
+    assert need(8192, 16, 0) > 0
+    for window in (2 ** 31 - 1, 2 ** 31, 2 ** 62, 2 ** 63 - 17, 2 ** 63 - 16, 2 ** 63 - 1):
+        assert need(8192, 16, window) == need(8192, 16, 0)
+    assert need(8192, 16, 1000) == need(-(-1016 // 16), 16, 0)
+    most = 2 ** 31 - 2
+    assert need(most, most, 0, 64) == need(2 ** 20, 2 ** 11, 0, 64) > 0
+
+
 def test_the_oracle_skips_bad_pages_and_empty_rows():
     g = torch.Generator().manual_seed(4)
     q = torch.randn(3, 2, 64, generator=g)
