@@ -697,25 +697,26 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// A paged cache [pages, page_size, heads, dim] and, in 8 bits, its scales [pages, page_size, heads].
+// A paged cache [pages, page_size, heads, dim] and, in 8 bits, its scales [pages, page_size, heads]. The kernels access
+// 8 elements of 16 bits at once, of 8 bits 8 (the store) or 16 (decode): `fp8_unit`.
 struct CacheArg {
   ako4x_kv_cache c = {};
-  CacheArg(const char* op, const Tensor& t, const Tensor& scale, ScalarType rows) {
+  CacheArg(const char* op, const Tensor& t, const Tensor& scale, ScalarType rows, int64_t fp8_unit) {
     if (t.dim() != 4) fail(std::string(op) + ": caches must be [pages, page_size, heads, dim]");
     const bool fp8 = t.scalar_type() == at::kFloat8_e4m3fn;
     if (!fp8 && t.scalar_type() != rows) fail(std::string(op) + ": caches must be of the rows' type or e4m3");
     if (fp8 != scale.defined()) fail(std::string(op) + ": e4m3 caches, and only those, come with scales");
     if (fp8 && !(scale.scalar_type() == at::kFloat && shape_is(scale, {t.size(0), t.size(1), t.size(2)})))
       fail(std::string(op) + ": scales must be fp32 [pages, page_size, heads]");
-    const int64_t to = fp8 ? 16 : 8;   // elements in 16 bytes
+    const int64_t to = fp8 ? fp8_unit : 8, bytes = fp8 ? to : 16;
     int64_t st[3];
     bool fits = t.size(3) <= 1 || t.stride(3) == 1;
     for (int d = 0; d < 3; ++d) {
       st[d] = t.size(d) > 1 ? t.stride(d) : 0;
       fits = fits && st[d] % to == 0;
     }
-    if (t.numel() > 0 && (!fits || ((uintptr_t)t.data_ptr() & 15)))
-      fail(std::string(op) + ": caches need a contiguous last dimension and strides of whole 16 bytes");
+    if (t.numel() > 0 && (!fits || ((uintptr_t)t.data_ptr() & (bytes - 1))))
+      fail(std::string(op) + ": caches need a contiguous last dimension and strides of whole " + std::to_string(bytes) + " bytes");
     c.data = t.data_ptr();
     c.page_stride = st[0];
     c.slot_stride = st[1];
@@ -746,7 +747,7 @@ PyObject* qk_norm_rope_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const float eps = (float)number(a[12]);
   Rotation rot(op, a[5], a[6], a[13], a[14], tokens, dim);
   need(is_index(slots0) && slots0.dim() == 1 && slots0.size(0) == tokens, "qk_norm_rope: slot_mapping must be int32 or int64 [tokens]");
-  const CacheArg kca(op, kc, ks, q0.scalar_type()), vca(op, vc, vs, q0.scalar_type());
+  const CacheArg kca(op, kc, ks, q0.scalar_type(), 8), vca(op, vc, vs, q0.scalar_type(), 8);
   need(kc.sizes() == vc.sizes() && kc.scalar_type() == vc.scalar_type() && kc.size(2) == k0.size(1) && kc.size(3) == dim && kc.size(1) >= 1,
        "qk_norm_rope: caches must be [pages, page_size, k's heads, dim], of one type");
   OneDevice dev(op, {&q0, &k0, &v0, &qw, &kw, &rot.positions, &rot.freq, &slots0, &kc, &vc, &ks, &vs});
@@ -779,7 +780,7 @@ PyObject* paged_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t window = a[8] == Py_None ? 0 : integer(a[8]);
   need(q0.dim() == 3 && (q0.size(2) == 64 || q0.size(2) == 128 || q0.size(2) == 256), "paged_decode: q must be [batch, heads, 64, 128 or 256]");
   need(q0.scalar_type() == at::kBFloat16 || q0.scalar_type() == at::kHalf, "paged_decode: q must be bf16 or fp16");
-  const CacheArg kca(op, kc, ks, q0.scalar_type()), vca(op, vc, vs, q0.scalar_type());
+  const CacheArg kca(op, kc, ks, q0.scalar_type(), 16), vca(op, vc, vs, q0.scalar_type(), 16);
   const int64_t batch = q0.size(0), hq = q0.size(1), dim = q0.size(2), pages = kc.size(0), page_size = kc.size(1), hk = kc.size(2);
   need(vc.sizes() == kc.sizes() && vc.scalar_type() == kc.scalar_type() && kc.size(3) == dim && page_size >= 1,
        "paged_decode: caches must be [pages, page_size, kv_heads, dim], of one type");

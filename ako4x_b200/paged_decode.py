@@ -12,6 +12,7 @@ def run(q, k_cache, v_cache, block_table, seq_lens, sm_scale, k_scale=None, v_sc
     [pages, page_size, kv_heads] (``qk_norm_rope.run_to_cache`` writes both); token t of sequence b in page
     ``block_table[b, t // page_size]`` (int32), slot ``t % page_size``; ``seq_lens`` int32 [batch] with the new token
     counted in; ``window`` > 0: only the last so many tokens are visible.
+    Any strides of the caches of whole 16 bytes with a contiguous last dimension will do.
 
     Returns (o like q, lse fp32 [batch, q_heads], the base-2 log of the sum of exp(sm_scale q.k)). A sequence that
     sees nothing gives o = 0, lse = -inf; tokens whose page id is outside the cache are not visible."""

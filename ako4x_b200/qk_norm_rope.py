@@ -20,7 +20,7 @@ def run_to_cache(q, k, v, q_weight, k_weight, positions, inv_freq, slot_mapping,
     (-1) leaves that token out of it. A weight of None leaves that norm out: rotation and store alone.
 
     The caches are of the rows' type, or e4m3 with fp32 scales ``k_scale`` / ``v_scale`` [pages, page_size, k_heads],
-    one per row: amax / 448, or 1 where amax <= 1e-10. Any strides of whole 16 bytes with a contiguous
+    one per row: amax / 448, or 1 where amax <= 1e-10. Any strides of whole 16 bytes (e4m3: 8) with a contiguous
     last dimension will do."""
     return _cabi.native().qk_norm_rope_cache(q, k, v, q_weight, k_weight, positions, inv_freq, slot_mapping, k_cache, v_cache,
                                              k_scale, v_scale, eps, interleaved, attention_factor)

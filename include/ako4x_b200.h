@@ -342,8 +342,8 @@ typedef struct {
 } ako4x_head_rows;
 
 /* Keys (or values) of a paged cache, [num_pages, page_size, heads, dim] with the last dimension contiguous
- * and any strides (in elements; data and strides multiples of 16 bytes): pages of whole tokens, pages of whole
- * heads, keys and values side by side. In an e4m3 cache the value of an element is e4m3 * scale, with
+ * and any strides (in elements; data and strides multiples of 16 bytes, or of 8 for the store into an e4m3
+ * cache): pages of whole tokens, pages of whole heads, keys and values side by side. In an e4m3 cache the value of an element is e4m3 * scale, with
  * one fp32 scale per slot and head, [num_pages, page_size, heads] of strides of its own; otherwise NULL. */
 typedef struct {
   void* data;

@@ -82,6 +82,20 @@ def test_cache_refusals(built_lib):
     _refused(call(vc=turned), "contiguous last dimension")
 
 
+@pytest.mark.parametrize("dim", [8, 24, 72, 104, 136, 248])
+def test_e4m3_caches_of_rows_of_8_bytes(built_lib, dim):
+    """Rows of any multiple of 8 are stored; decode reads 16 bytes at once."""
+    q, k, pos, f = _rows(dim=dim)
+    w, slots = torch.ones(dim, dtype=BF16), torch.arange(3, dtype=torch.int32)
+    c, sc = torch.zeros(2, 16, 2, dim).to(E4M3), torch.ones(2, 16, 2)
+    _refused(lambda: qk_norm_rope.run_to_cache(q, k, k, w, w, pos, f, slots, c, c, sc, sc), "CUDA")
+    odd = torch.zeros(2, 16, 2, dim + 4).to(E4M3)[..., :dim]
+    _refused(lambda: qk_norm_rope.run_to_cache(q, k, k, w, w, pos, f, slots, odd, c, sc, sc), "8 bytes")
+    apart = torch.zeros(2, 16, 2, 72).to(E4M3)[..., :64]
+    _refused(lambda: paged_decode.run(torch.zeros(2, 8, 64, dtype=BF16), apart, apart, torch.zeros(2, 3, dtype=torch.int32),
+                                      torch.ones(2, dtype=torch.int32), 0.1, sc, sc), "16 bytes")
+
+
 def test_rows_c_status(built_lib):
     L = _cabi.lib()
     raw = ctypes.create_string_buffer(4096)
