@@ -606,6 +606,8 @@ struct Rotation {
       fail(std::string(op) + ": positions must be int32 or int64 [tokens]");
     if (!(freq.scalar_type() == at::kFloat && freq.dim() == 1 && rotary <= dim))
       fail(std::string(op) + ": inv_freq must be fp32 [rotary_dim / 2] with rotary_dim <= dim");
+  }
+  void lay() {   // behind the check of the devices, as every copy
     positions = dense(positions);
     freq = dense(freq);
   }
@@ -622,19 +624,24 @@ void check_rows(const char* op, const Tensor& q, const Tensor& k, const char* na
     fail(std::string(op) + ": dim must be a multiple of 8 from 8 to 256");
 }
 // Both weights [dim], of the rows' type or fp32 both.
-bool check_weights(const char* op, Tensor& qw, Tensor& kw, const Tensor& q) {
+bool check_weights(const char* op, const Tensor& qw, const Tensor& kw, const Tensor& q) {
   bool fp32 = false, any = false;
-  for (Tensor* w : {&qw, &kw}) {
+  for (const Tensor* w : {&qw, &kw}) {
     if (!w->defined()) continue;
     if (!(w->dim() == 1 && w->size(0) == q.size(2) && (w->scalar_type() == q.scalar_type() || w->scalar_type() == at::kFloat)))
       fail(std::string(op) + ": weights must be [dim], of the rows' type or fp32");
     if (any && fp32 != (w->scalar_type() == at::kFloat)) fail(std::string(op) + ": weights must be of one type");
     fp32 = w->scalar_type() == at::kFloat;
     any = true;
+  }
+  return fp32;
+}
+void lay_weights(Tensor& qw, Tensor& kw) {
+  for (Tensor* w : {&qw, &kw}) {
+    if (!w->defined()) continue;
     *w = dense(*w);
     if ((uintptr_t)w->data_ptr() & 15) *w = w->clone();   // a view into something else: the kernels read 16 bytes at once
   }
-  return fp32;
 }
 
 // (q, k or None, positions, inv_freq, interleaved, attention_factor)
@@ -647,6 +654,7 @@ PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t tokens = q0.size(0), dim = q0.size(2);
   Rotation rot("rope", a[2], a[3], a[4], a[5], tokens, dim);
   OneDevice dev("rope", {&q0, &k0, &rot.positions, &rot.freq});
+  rot.lay();
   HeadRows q(q0), k;
   Tensor qo = empty(q0.sizes(), q0.scalar_type(), q0), ko;
   if (k0.defined()) {
@@ -683,6 +691,8 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const float eps = (float)number(a[6]);
   Rotation rot("qk_norm_rope", a[4], a[5], a[7], a[8], tokens, dim);
   OneDevice dev("qk_norm_rope", {&q0, &k0, &qw, &kw, &rot.positions, &rot.freq});
+  rot.lay();
+  lay_weights(qw, kw);
   HeadRows q(q0), k(k0);
   Tensor qo = empty(q0.sizes(), q0.scalar_type(), q0), ko = empty(k0.sizes(), k0.scalar_type(), k0);
   void *pp = rot.positions.data_ptr(), *fp = rot.freq.data_ptr(), *qp = qo.data_ptr(), *kp = ko.data_ptr(), *qwp = qw.data_ptr(),
@@ -751,6 +761,8 @@ PyObject* qk_norm_rope_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
   need(kc.sizes() == vc.sizes() && kc.scalar_type() == vc.scalar_type() && kc.size(2) == k0.size(1) && kc.size(3) == dim && kc.size(1) >= 1,
        "qk_norm_rope: caches must be [pages, page_size, k's heads, dim], of one type");
   OneDevice dev(op, {&q0, &k0, &v0, &qw, &kw, &rot.positions, &rot.freq, &slots0, &kc, &vc, &ks, &vs});
+  rot.lay();
+  lay_weights(qw, kw);
   const Tensor slots = dense(slots0);
   HeadRows q(q0), k(k0), v(v0);
   Tensor qo = empty(q0.sizes(), q0.scalar_type(), q0);

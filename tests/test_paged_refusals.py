@@ -82,6 +82,26 @@ def test_cache_refusals(built_lib):
     _refused(call(vc=turned), "contiguous last dimension")
 
 
+def test_nothing_is_copied_before_the_devices_are_checked(built_lib):
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Seen(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            ops.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    q, k, _, _ = _rows(dim=64)
+    pos, f, w = torch.arange(6, dtype=torch.int32)[::2], torch.ones(64)[::2], torch.ones(128, dtype=BF16)[::2]
+    off = torch.ones(65, dtype=BF16)[1:]
+    slots, kc = torch.arange(3, dtype=torch.int32), torch.zeros(2, 16, 2, 64, dtype=BF16)
+    for call in (lambda: rope.run(q, k, pos, f), lambda: qk_norm_rope.run(q, k, w, off, pos, f),
+                 lambda: qk_norm_rope.run_to_cache(q, k, k, off, w, pos, f, slots, kc, kc)):
+        ops = []
+        with Seen():
+            _refused(call, "CUDA")
+        assert ops == []
+
+
 @pytest.mark.parametrize("dim", [8, 24, 72, 104, 136, 248])
 def test_e4m3_caches_of_rows_of_8_bytes(built_lib, dim):
     """Rows of any multiple of 8 are stored; decode reads 16 bytes at once."""
