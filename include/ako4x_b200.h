@@ -385,7 +385,8 @@ int ako4x_qk_norm_rope_cache(const ako4x_head_rows* q, const ako4x_head_rows* k,
  * head h reads KV head h / (q_heads / kv_heads). Token t of sequence b lies in page block_table[b, t / page_size],
  * slot t % page_size; seq_lens[b] tokens (at most max_pages * page_size are read), of which the last `window` are
  * visible (0: all). Tokens of a page id outside [0, num_pages) are not visible. o like q, lse fp32 [batch,
- * q_heads] = log2(sum exp(sm_scale q.k)); a sequence that sees nothing gives o = 0, lse = -inf. */
+ * q_heads] = log2(sum exp(sm_scale q.k)); a sequence that sees nothing gives o = 0, lse = -inf. A visible key that scores
+ * -inf weighs 0, and 0 times an infinite value or a NaN is NaN. */
 size_t ako4x_paged_decode_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim,
                                           int64_t max_pages, int64_t page_size, int64_t window);
 int ako4x_paged_decode(const void* q, const ako4x_kv_cache* k_cache, const ako4x_kv_cache* v_cache,

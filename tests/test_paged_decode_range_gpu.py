@@ -151,3 +151,21 @@ def test_an_infinite_value_far_below_the_others(built_lib, lens, hk, group, dim,
     o = o.cpu().double()
     assert torch.equal(o[..., 3], ro[..., 3]) and torch.equal(o[..., 8], ro[..., 8])
     assert int(torch.isfinite(o).sum()) == o.numel() // dim * (dim - 2)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("lens,hk,group,dim,ps", LAYOUTS)
+def test_a_key_that_scores_minus_infinity_weighs_zero(built_lib, lens, hk, group, dim, ps, dtype):
+    """A finite value of it is left out; 0 times another one is NaN, in its feature."""
+    a = make(lens, hk, group, dim, dtype, dtype, ps, seed=dim + 4)
+    a["q"] = a["q"].abs() + 0.125
+    for b, n in enumerate(lens):
+        a["k_cache"][at(a, b, n // 2)] = float("-inf")
+    want = run_check(a)
+    for b, n in enumerate(lens):
+        a["v_cache"][at(a, b, n // 2)][..., 3], a["v_cache"][at(a, b, n // 2)][..., 8] = float("inf"), float("nan")
+    o, lse = paged_decode.run(**on_gpu(a))
+    bad = torch.zeros_like(o, dtype=torch.bool)
+    bad[..., 3] = bad[..., 8] = True
+    assert torch.equal(torch.isnan(o), bad) and torch.equal(lse, want[1])
+    assert torch.equal(o[~bad], want[0][~bad])
