@@ -85,11 +85,8 @@ struct Pair<__half> {
   static __device__ __forceinline__ float one(const void* p) { return __half2float(*(const __half*)p); }
 };
 
-using F2 = float2;
-__device__ __forceinline__ F2 f2(float a, float b) { return make_float2(a, b); }
-__device__ __forceinline__ float2 both(F2 a) { return a; }
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) { return make_float2(fmaf(a.x, b.x, c.x), fmaf(a.y, b.y, c.y)); }
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) { return make_float2(a.x * b.x, a.y * b.y); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return make_float2(fmaf(a.x, b.x, c.x), fmaf(a.y, b.y, c.y)); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return make_float2(a.x * b.x, a.y * b.y); }
 
 __device__ __forceinline__ float max_nan(float a, float b) {   // a NaN stays
   float r;
@@ -218,7 +215,7 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == STAGED ? 4 : PE == 8 ? 
 
   const float2* cs_of = s_cs[warp] + (real ? mine : 0) * pitch;
   // Pairs (2i, 2i + 1) of the pieces' elements: z = inv (x A + x' B), where `mask` says so; inv x A elsewhere.
-  F2 A[2][PE / 2], B[2][PE / 2];
+  float2 A[2][PE / 2], B[2][PE / 2];
   unsigned mask = 0;
   auto tables = [&](const void* weight) {
     float w[2][PE];
@@ -246,8 +243,8 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == STAGED ? 4 : PE == 8 ? 
       }
 #pragma unroll
       for (int j = 0; j < PE / 2; ++j) {
-        A[h][j] = f2(w[h][2 * j], w[h][2 * j + 1]);
-        B[h][j] = f2(0.f, 0.f);
+        A[h][j] = make_float2(w[h][2 * j], w[h][2 * j + 1]);
+        B[h][j] = make_float2(0.f, 0.f);
       }
     }
     mask = 0;
@@ -257,10 +254,10 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == STAGED ? 4 : PE == 8 ? 
 #pragma unroll
         for (int j = 0; j < PE / 2; ++j) {
           const float4 cs = *reinterpret_cast<const float4*>(cs_of + e0 + 2 * j);
-          A[0][j] = f2(w[0][2 * j] * cs.x, w[0][2 * j + 1] * cs.z);
-          A[1][j] = f2(w[1][2 * j] * cs.x, w[1][2 * j + 1] * cs.z);
-          B[0][j] = f2(-w[1][2 * j] * cs.y, -w[1][2 * j + 1] * cs.w);
-          B[1][j] = f2(w[0][2 * j] * cs.y, w[0][2 * j + 1] * cs.w);
+          A[0][j] = make_float2(w[0][2 * j] * cs.x, w[0][2 * j + 1] * cs.z);
+          A[1][j] = make_float2(w[1][2 * j] * cs.x, w[1][2 * j + 1] * cs.z);
+          B[0][j] = make_float2(-w[1][2 * j] * cs.y, -w[1][2 * j + 1] * cs.w);
+          B[1][j] = make_float2(w[0][2 * j] * cs.y, w[0][2 * j + 1] * cs.w);
         }
       }
     } else if (PARTNER == SAME_PIECE) {
@@ -272,8 +269,8 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == STAGED ? 4 : PE == 8 ? 
           if (e < p.rotary) {
             const float2 cs = cs_of[e / 2];
             mask |= 1u << (PE / 2 * h + j);
-            A[h][j] = f2(w[h][2 * j] * cs.x, w[h][2 * j + 1] * cs.x);
-            B[h][j] = f2(-w[h][2 * j + 1] * cs.y, w[h][2 * j] * cs.y);
+            A[h][j] = make_float2(w[h][2 * j] * cs.x, w[h][2 * j + 1] * cs.x);
+            B[h][j] = make_float2(-w[h][2 * j + 1] * cs.y, w[h][2 * j] * cs.y);
           }
         }
     }
@@ -324,47 +321,43 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == STAGED ? 4 : PE == 8 ? 
 #pragma unroll 1
     for (; it < stop; ++it, head += slots, to0 += out_step, to1 += out_step) {
       const bool live = store && head < heads;
-      F2 y[2][PE / 2];
+      float2 y[2][PE / 2];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int j = 0; j < PE / 2; ++j) {
-          const float2 x = Pair<T>::get(word(raw[0][h], j));
-          y[h][j] = f2(x.x, x.y);
-        }
+        for (int j = 0; j < PE / 2; ++j) y[h][j] = Pair<T>::get(word(raw[0][h], j));
       next();
       if (p.ragged) {                 // pieces behind the row's end
 #pragma unroll
         for (int h = 0; h < 2; ++h)
           if (!(h ? in1 : in0)) {
 #pragma unroll
-            for (int j = 0; j < PE / 2; ++j) y[h][j] = f2(0.f, 0.f);
+            for (int j = 0; j < PE / 2; ++j) y[h][j] = make_float2(0.f, 0.f);
           }
       }
       if (turn) {
-        F2 o[2][PE / 2];
+        float2 o[2][PE / 2];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int j = 0; j < PE / 2; ++j) {
             if (PARTNER == OTHER_PIECE) o[h][j] = y[1 - h][j];
-            if (PARTNER == SAME_PIECE) o[h][j] = f2(y[h][j].y, y[h][j].x);
+            if (PARTNER == SAME_PIECE) o[h][j] = make_float2(y[h][j].y, y[h][j].x);
           }
         float inv = 1.f;
         if (weight) {
-          F2 ss = mul2(y[0][0], y[0][0]), st = mul2(y[1][0], y[1][0]);
+          float2 ss = mul2(y[0][0], y[0][0]), st = mul2(y[1][0], y[1][0]);
 #pragma unroll
           for (int j = 1; j < PE / 2; ++j) {
             ss = fma2(y[0][j], y[0][j], ss);
             st = fma2(y[1][j], y[1][j], st);
           }
-          const float2 a = both(ss), b = both(st);
-          float sum = (a.x + a.y) + (b.x + b.y);
+          float sum = (ss.x + ss.y) + (st.x + st.y);
 #pragma unroll
           for (int m = LANES / 2; m >= 1; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
           inv = rsqrtf(fmaf(sum, p.inv_dim, p.eps));
         }
-        F2 z[2][PE / 2];
+        float2 z[2][PE / 2];
         if (PARTNER == STAGED) {            // a pair to a lane, and back
           float* staged = s_row[warp][lane32 / LANES];
 #pragma unroll
@@ -373,7 +366,7 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == STAGED ? 4 : PE == 8 ? 
             for (int j = 0; j < PE / 2; ++j) {
               z[h][j] = mul2(y[h][j], A[h][j]);
               const int e = (h ? e1 : e0) + 2 * j;
-              if (e < p.rotary) *reinterpret_cast<F2*>(staged + e) = z[h][j];
+              if (e < p.rotary) *reinterpret_cast<float2*>(staged + e) = z[h][j];
             }
           __syncwarp();
           for (int i = lane; i < half; i += LANES) {
@@ -388,7 +381,7 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == STAGED ? 4 : PE == 8 ? 
 #pragma unroll
             for (int j = 0; j < PE / 2; ++j) {
               const int e = (h ? e1 : e0) + 2 * j;
-              if (e < p.rotary) z[h][j] = *reinterpret_cast<const F2*>(staged + e);
+              if (e < p.rotary) z[h][j] = *reinterpret_cast<const float2*>(staged + e);
             }
           __syncwarp();                     // read before the next row is put there
         } else if (all) {
@@ -405,7 +398,7 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == STAGED ? 4 : PE == 8 ? 
               if (mask >> (PE / 2 * h + j) & 1) z[h][j] = fma2(o[h][j], B[h][j], z[h][j]);
             }
         }
-        const F2 by = f2(inv, inv);
+        const float2 by = make_float2(inv, inv);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -418,7 +411,7 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == STAGED ? 4 : PE == 8 ? 
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int j = 0; j < PE / 2; ++j) {
-            const float2 x = both(y[h][j]);
+            const float2 x = y[h][j];
             top = max_nan(top, max_nan(fabsf(x.x), fabsf(x.y)));
           }
 #pragma unroll
@@ -429,7 +422,7 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == STAGED ? 4 : PE == 8 ? 
           uint32_t w[PE / 4] = {};
 #pragma unroll
           for (int j = 0; j < PE / 2; ++j) {
-            const float2 x = both(y[h][j]);
+            const float2 x = y[h][j];
             const uint32_t pair = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(x.x, sc), __fdiv_rn(x.y, sc)), __NV_SATFINITE, __NV_E4M3);
             w[j >> 1] |= pair << (16 * (j & 1));
           }
@@ -443,7 +436,7 @@ __global__ void __launch_bounds__(WARPS * 32, PARTNER == STAGED ? 4 : PE == 8 ? 
           uint32_t w[PE / 2];
 #pragma unroll
           for (int j = 0; j < PE / 2; ++j) {
-            const float2 x = both(y[h][j]);
+            const float2 x = y[h][j];
             w[j] = Pair<T>::put(x.x, x.y);
           }
           if (live && (h ? in1 : in0)) Words<PE>::put_once(h ? to1 : to0, w);
