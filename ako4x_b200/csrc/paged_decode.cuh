@@ -136,8 +136,8 @@ __device__ __forceinline__ void widen(uint32_t w, uint32_t& low, uint32_t& high)
       : "r"(w));
 }
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }   // -126 .. 127
-// e with 2^e <= x < 2^(e + 1), within [-120, 120]
-__device__ __forceinline__ int exponent(float x) { return min(max(((int)(__float_as_uint(x) >> 23) & 0xff) - 127, -120), 120); }
+// e with 2^e <= x < 2^(e + 1), -112 at least
+__device__ __forceinline__ int exponent(float x) { return min(max(((int)(__float_as_uint(x) >> 23) & 0xff) - 127, -112), 127); }
 
 // A weight p >= 0 as hi + lo, both positive where p is: p cut to its leading bits, and the rest with 2^-20 of p.
 __device__ __forceinline__ void two_pieces(float p0, float p1, uint32_t& hi, uint32_t& lo) {
@@ -339,8 +339,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
     }
     float qs0 = p.scale_log2, qs1 = p.scale_log2;   // of heads 2t and 2t + 1
     if (FP8 && std::is_same<T, __nv_bfloat16>::value) {
-      // bf16 to fp16: times the power of two that brings the head's largest element to [1, 2). What falls below
-      // the fp16 range is off by 2^-25 of that.
+      // bf16 to fp16: times the power of two that brings the head's largest element to [2^14, 2^15). Elements down to
+      // 2^-31 of that are exact, what is below is off by 2^-39 of it at most.
       float top = 0.f;
 #pragma unroll
       for (int i = 0; i < KS; ++i)
@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const int e = exponent(top);
-      const float down = power_of_two(-e), back = power_of_two(e);
+      const float down = power_of_two(14 - e), back = power_of_two(e - 14);
 #pragma unroll
       for (int i = 0; i < KS; ++i)
 #pragma unroll

@@ -17,5 +17,6 @@ def run(q, k_cache, v_cache, block_table, seq_lens, sm_scale, k_scale=None, v_sc
     Returns (o like q, lse fp32 [batch, q_heads], the base-2 log of the sum of exp(sm_scale q.k)). A sequence that
     sees nothing gives o = 0, lse = -inf; tokens whose page id is outside the cache are not visible, and what lies there, or
     behind a sequence, does not matter. A visible key that scores minus infinity weighs 0 like one that is not visible, but 0
-    times an infinite value, or a NaN, is NaN."""
+    times an infinite value, or a NaN, is NaN. bf16 queries over an e4m3 cache: elements of q that are 2^31 times smaller
+    than the largest of their head lose bits (2^-39 of that)."""
     return _cabi.native().paged_decode(q, k_cache, v_cache, block_table, seq_lens, sm_scale, k_scale, v_scale, window)

@@ -3,7 +3,9 @@ against the formula in 64 bits.
 
 Tolerances as in the tests of ordinary values: the output's own rounding (half a step, finfo.eps / 2 of its value), and,
 relative to the weighted mean magnitude of the values, 2^-15 for the two pieces of a weight, n / 16 + 64 roundings of
-fp32 for the sums, dim 2^-24 A for a score of magnitude A, 2^-21 for exp2. None of them has an absolute part but the end of
+fp32 for the sums, dim 2^-24 A for a score of magnitude A, 2^-21 for exp2. Queries in bf16 meet e4m3 keys in fp16, a
+head's largest element at 2^14 to 2^15: the smallest step of fp16, 2^-24, is then 2^-38 of it at most, so that every element of q is off by
+half of that, 2^-39 of the largest, and a score by that times the sum of its key's magnitudes. None of them has an absolute part but the end of
 the output's type: 2^-25 in fp16, 2^-134 in bf16."""
 import pytest
 import torch
@@ -20,6 +22,9 @@ def check(a, o, lse, **more):
     ro, rlse, size, score = oracle.paged.paged_decode(**{**a, **more})
     dim, n = a["q"].shape[2], max(int(x) for x in a["seq_lens"])
     rel = (n / 16 + 64) * 2.0 ** -24 + dim * 2.0 ** -24 * score + 2.0 ** -21
+    if a["k_cache"].dtype == E4M3 and o.dtype == BF16:
+        key = (a["k_cache"].double().abs().sum(-1) * a["k_scale"].double()).max()
+        rel = rel + 2.0 ** -39 * a["q"].double().abs().amax(-1) * key * a["sm_scale"]
     end = 2.0 ** -25 if o.dtype == FP16 else 2.0 ** -134
     tol = torch.finfo(o.dtype).eps / 2 * (1 + 2.0 ** -8) * ro.abs() + (rel + 2.0 ** -15)[..., None] * size + end
     o = o.cpu().double()
@@ -110,6 +115,26 @@ def test_values_near_the_end_of_bf16(built_lib, lens, hk, group, dim, ps):
     """No sum of weights and values is above 2^126: 700 times 448 times 2^107."""
     a = make([min(n, 700) for n in lens], hk, group, dim, BF16, E4M3, ps, seed=dim + 3)
     a["v_scale"] = a["v_scale"] * 50 * 2.0 ** 107
+    run_check(a)
+
+
+@pytest.mark.parametrize("octaves", [10, 20, 28])
+@pytest.mark.parametrize("lens,hk,group,dim,ps", LAYOUTS)
+def test_a_feature_of_q_far_above_the_others(built_lib, lens, hk, group, dim, ps, octaves):
+    """That no key has: the scores come from the others."""
+    a = make(lens, hk, group, dim, BF16, E4M3, ps, seed=dim + octaves + 1)
+    a["q"][..., 7] = 2.0 ** octaves
+    a["k_cache"][..., 7] = 0
+    run_check(a)
+
+
+@pytest.mark.parametrize("power", [-119, -110, -60, 60, 124])
+@pytest.mark.parametrize("lens,hk,group,dim,ps", LAYOUTS)
+def test_queries_of_any_size(built_lib, lens, hk, group, dim, ps, power):
+    """Against scales of the keys that make ordinary scores of them."""
+    a = make(lens, hk, group, dim, BF16, E4M3, ps, seed=dim + 5)
+    a["q"] = (a["q"].float().clamp(-7, 7) * 2.0 ** power).to(BF16)
+    a["k_scale"] = a["k_scale"] * 2.0 ** -power
     run_check(a)
 
 
