@@ -49,12 +49,15 @@ def frequencies(rotary_dim, base=10000.0, scaling="none", factor=1.0, original_l
             raise _cabi.Ako4xError("rope: yarn scaling needs original_length")
         if not base > 1:
             raise _cabi.Ako4xError("rope: yarn scaling needs a base above 1")
+        if not beta_fast >= beta_slow > 0:
+            raise _cabi.Ako4xError("rope: yarn scaling needs beta_fast >= beta_slow > 0")
 
         def index_of(turns):   # of the frequency that turns so often
             return half * math.log(original_length / (2 * math.pi * turns)) / math.log(base)
 
         low, high = max(math.floor(index_of(beta_fast)), 0), min(math.ceil(index_of(beta_slow)), rotary_dim - 1)
         ramp = ((i - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
+        ramp[i > index_of(beta_slow)] = 1.0   # all of them, where the first one turns too seldom already
         f = base ** (-i / half) * (1.0 - ramp + ramp / factor)
         if factor > 1:
             attention_factor = 0.1 * math.log(factor) + 1.0

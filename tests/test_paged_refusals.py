@@ -184,6 +184,23 @@ def test_frequencies():
             rope.frequencies(device="cpu", **bad)
 
 
+@pytest.mark.parametrize("length,slow,fast,dim,base", [(6, 1.0, 32.0, 64, 1e4), (512, 100.0, 100.0, 64, 1e4), (4096, 1.0, 32.0, 8, 1e6), (4096, 1.0, 1.0, 128, 1e4),
+                                                       (1, 1.0, 32.0, 2, 1e4), (10 ** 9, 1.0, 32.0, 64, 1e4)])
+def test_yarn_keeps_and_divides_as_it_says(length, slow, fast, dim, base):
+    f, _ = rope.frequencies(dim, base=base, device="cpu")
+    y, _ = rope.frequencies(dim, base=base, scaling="yarn", factor=8.0, original_length=length, beta_fast=fast, beta_slow=slow, device="cpu")
+    turns = length * f.double() / (2 * math.pi)
+    assert torch.equal(y[turns > fast], f[turns > fast])
+    assert torch.allclose(y[turns < slow], f[turns < slow] / 8, rtol=1e-6)
+    assert (y <= f).all() and (y >= f / 8 * (1 - 1e-6)).all()
+
+
+def test_yarn_refusals():
+    for bad in (dict(beta_fast=0.5), dict(beta_slow=0.0), dict(beta_slow=-1.0), dict(beta_fast=float("nan"))):
+        with pytest.raises(_cabi.Ako4xError, match="beta"):
+            rope.frequencies(64, scaling="yarn", factor=4.0, original_length=4096, device="cpu", **bad)
+
+
 def test_the_oracles_rotation_is_one():
     """Lengths stay, and a rotation back by the negative positions undoes it."""
     g = torch.Generator().manual_seed(3)
