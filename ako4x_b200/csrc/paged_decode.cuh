@@ -14,14 +14,16 @@
 //   * V in registers like K, or, for e4m3 and for 256 features, two tiles of it in shared memory by asynchronous copies that a
 //     lane reads back itself (128 sequences in e4m3: all in registers 235 to 249 us, V in shared memory 218, K too 223;
 //     three of up to 131 072 with 256 features, K and V there: 35, V alone 31).
-//   * P goes in as two pieces of bf16, which have the exponents of fp32, so that a weight counts however small it is beside
+//   * P goes in as two pieces, of bf16, which have the exponents of fp32, so that a weight counts however small it is beside
 //     the others; both are positive for a positive weight, so that an infinite value stays infinite: hi = P cut to its leading bits,
 //     lo = the rest. One piece would put its own rounding beside the output's, and more of it the fewer keys there are.
 //   * Groups of four query heads and fewer leave half of the eight columns free: the second piece of P goes there, and the
 //     accumulators of the two halves are added at the end (64 sequences of up to 8 192 tokens 166 -> 161 us).
-//   * fp16: P V on tf32 (mma.m16n8k8), which holds P's pieces and fp16 values exactly. Two pieces of P in fp16 end at 2^-39
-//     of the largest weight, and where the key that has it has no value, what lies below is all there is. (64 sequences of up to
-//     8 192 tokens 156 us both ways, 28 heads over 4 84 in fp16, 87 on tf32.)
+//   * fp16: the pieces of P are fp16, the largest weight at 2^15 (the sum too), as long as a tile's weights are 2^-23 of that
+//     and more, which two pieces hold. Below, fp16's end at 2^-24 takes their bits, and where the key with the largest weight has
+//     no value they are all there is: such a tile takes tf32 (mma.m16n8k8), which holds the pieces of bf16 and fp16 values
+//     exactly. Three sequences of up to 131 072 tokens, seven heads over one of 256: 30.9 us, all on tf32 31.7; 64 of up to 8 192,
+//     28 heads over 4 of 128: 84.5 and 87 to 90.
 //   * e4m3 becomes fp16 exactly, NaN included (one conversion for a pair: 1.6 cycles of an SM for a word of each lane,
 //     against 3.6 by shifts to bf16; mma.m16n8k32 on e4m3 itself, with q in pieces, takes more instructions in all), and V
 //     goes on to bf16, exact too. The scale of a key multiplies its score, the scale of a value its weight: these products differ by as much
@@ -139,10 +141,24 @@ __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e 
 // e with 2^e <= x < 2^(e + 1), -112 at least
 __device__ __forceinline__ int exponent(float x) { return min(max(((int)(__float_as_uint(x) >> 23) & 0xff) - 127, -112), 127); }
 
-// A weight p >= 0 as hi + lo, both positive where p is: p cut to its leading bits, and the rest with 2^-20 of p.
-__device__ __forceinline__ void two_pieces(float p0, float p1, uint32_t& hi, uint32_t& lo) {
+// A weight p >= 0 as hi + lo, both positive where p is: in bf16 p cut to its leading bits, and the rest with 2^-20 of p.
+template <class T>
+__device__ __forceinline__ void two_pieces(float p0, float p1, uint32_t& hi, uint32_t& lo);
+template <>
+__device__ __forceinline__ void two_pieces<__nv_bfloat16>(float p0, float p1, uint32_t& hi, uint32_t& lo) {
   hi = __byte_perm(__float_as_uint(p0), __float_as_uint(p1), 0x7632);
   lo = ako::pack_bf16x2(fmaf(p0, 1.f + 0x1p-20f, -ako::bf16_lo(hi)), fmaf(p1, 1.f + 0x1p-20f, -ako::bf16_hi(hi)));
+}
+// In fp16 0, or LEAST and more: the rest is 2^-24 at least, 2^-16 of that.
+constexpr float LEAST = 0x1p-8f;
+template <>
+__device__ __forceinline__ void two_pieces<__half>(float p0, float p1, uint32_t& hi, uint32_t& lo) {
+  __half2 h = __halves2half2(__float2half_rz(p0), __float2half_rz(p1));
+  hi = *reinterpret_cast<uint32_t*>(&h);
+  const float2 c = __half22float2(h);
+  const float r0 = p0 > 0.f ? fmaxf(p0 - c.x, 0x1p-24f) : p0, r1 = p1 > 0.f ? fmaxf(p1 - c.y, 0x1p-24f) : p1;
+  __half2 l = __floats2half2_rn(r0, r1);
+  lo = *reinterpret_cast<uint32_t*>(&l);
 }
 // D (16 x 8) += A (16 x 8, row) B (8 x 8, column), both with eight bits of exponent and ten behind the point.
 __device__ __forceinline__ void mma_tf32(float (&d)[4], const float (&a)[4], float b0, float b1) {
@@ -191,7 +207,9 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
   constexpr int TT = blocks(D, FP8), TILE = BLOCK * TT, R = 2 * TT;   // R: tokens of a lane in a tile
   constexpr int SLOT = R * NJ * 512, PART = warp_bytes(D, FP8);      // V of a tile; what a warp has of shared memory
   using TM = typename std::conditional<FP8, __half, T>::type;   // operand type of Q K^T
-  constexpr bool WIDE = !FP8 && std::is_same<T, __half>::value;  // P V on tf32, otherwise on bf16
+  using TV = typename std::conditional<FP8, __nv_bfloat16, T>::type;   // and of P V
+  constexpr bool HALF = std::is_same<TV, __half>::value;
+  constexpr float LIFT = HALF ? 15.f : 0.f;
   __shared__ int s_scan[6];
   extern __shared__ __align__(16) unsigned char s_ring[];   // [warp]: its tiles, and then its part
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -468,8 +486,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
       }
 #pragma unroll
       for (int i = 0; i < R; ++i) {
-        e[i][0] = ako::fast_exp2(e[i][0] - m0);
-        e[i][1] = ako::fast_exp2(e[i][1] - m1);
+        e[i][0] = ako::fast_exp2(e[i][0] - m0 + LIFT);
+        e[i][1] = ako::fast_exp2(e[i][1] - m1 + LIFT);
         l0 += e[i][0];
         l1 += e[i][1];
       }
@@ -493,35 +511,27 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
         }
       }
       uint32_t bh[R], bl[R];
+      auto pieces = [&](auto&& cut) {
 #pragma unroll
-      for (int i = 0; i < R; ++i) {
-        two_pieces(e[i][0], e[i][1], bh[i], bl[i]);
-        if (FOLD) {
-          bh[i] = ako::movmatrix_trans(t < 2 ? bh[i] : bl[i]);
-        } else {
-          bh[i] = ako::movmatrix_trans(bh[i]);
-          bl[i] = ako::movmatrix_trans(bl[i]);
+        for (int i = 0; i < R; ++i) {
+          cut(e[i][0], e[i][1], bh[i], bl[i]);
+          if (FOLD) {
+            bh[i] = ako::movmatrix_trans(t < 2 ? bh[i] : bl[i]);
+          } else {
+            bh[i] = ako::movmatrix_trans(bh[i]);
+            bl[i] = ako::movmatrix_trans(bl[i]);
+          }
         }
-      }
+      };
+      auto each_step = [&](auto&& put) {               // put(accumulators, V^T of 16 features and 16 tokens, which of the tile's)
 #pragma unroll
-      for (int j = 0; j < NJ; ++j)
+        for (int j = 0; j < NJ; ++j)
 #pragma unroll
-        for (int u = 0; u < TT; ++u) {
-          const uint4 x = RINGED ? lds16(at_slot + (2 * u * NJ + j) * 512) : vc[RINGED ? 0 : 2 * u][RINGED ? 0 : j];
-          const uint4 y = RINGED ? lds16(at_slot + ((2 * u + 1) * NJ + j) * 512) : vc[RINGED ? 0 : 2 * u + 1][RINGED ? 0 : j];
+          for (int u = 0; u < TT; ++u) {
+            const uint4 x = RINGED ? lds16(at_slot + (2 * u * NJ + j) * 512) : vc[RINGED ? 0 : 2 * u][RINGED ? 0 : j];
+            const uint4 y = RINGED ? lds16(at_slot + ((2 * u + 1) * NJ + j) * 512) : vc[RINGED ? 0 : 2 * u + 1][RINGED ? 0 : j];
 #pragma unroll
-          for (int i = 0; i < (FP8 ? 4 : 2); ++i) {
-            float(&d)[4] = acc[(FP8 ? 4 : 2) * j + i];
-            if (WIDE) {                              // eight tokens at a time: as k = t and t + 4 the tokens 2t and 2t + 1
-#pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                const uint4& z = c ? y : x;
-                const float2 v0 = unpack_half(ako::movmatrix_trans(word(z, 2 * i))), v1 = unpack_half(ako::movmatrix_trans(word(z, 2 * i + 1)));
-                const float a[4] = {v0.x, v1.x, v0.y, v1.y};
-                if (!FOLD) mma_tf32(d, a, ako::bf16_lo(bl[2 * u + c]), ako::bf16_hi(bl[2 * u + c]));
-                mma_tf32(d, a, ako::bf16_lo(bh[2 * u + c]), ako::bf16_hi(bh[2 * u + c]));
-              }
-            } else {
+            for (int i = 0; i < (FP8 ? 4 : 2); ++i) {
               uint32_t a[4];
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
@@ -537,11 +547,39 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
                   a[2 * c + 1] = ako::movmatrix_trans(word(z, 2 * i + 1));
                 }
               }
-              if (!FOLD) ako::mma_bf16_16816(d, a, bl[2 * u], bl[2 * u + 1]);
-              ako::mma_bf16_16816(d, a, bh[2 * u], bh[2 * u + 1]);
+              put(acc[(FP8 ? 4 : 2) * j + i], a, u);
             }
           }
-        }
+      };
+      auto multiply = [&](float (&d)[4], const uint32_t (&a)[4], int u) {
+        if (!FOLD) mma<TV>(d, a, bl[2 * u], bl[2 * u + 1]);
+        mma<TV>(d, a, bh[2 * u], bh[2 * u + 1]);
+      };
+      bool small = false;
+      if (HALF) {
+        float least = now[0] ? fminf(e[0][0], e[0][1]) : INFINITY;
+#pragma unroll
+        for (int i = 1; i < R; ++i) least = now[i] ? fminf(least, fminf(e[i][0], e[i][1])) : least;
+        small = __any_sync(0xffffffffu, least < LEAST);
+      }
+      if (!HALF) {
+        pieces(two_pieces<__nv_bfloat16>);
+        each_step(multiply);
+      } else if (!small) {
+        pieces(two_pieces<__half>);
+        each_step(multiply);
+      } else {
+        pieces(two_pieces<__nv_bfloat16>);
+        each_step([&](float (&d)[4], const uint32_t (&a)[4], int u) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {                // eight tokens at a time: as k = t and t + 4 the tokens 2t and 2t + 1
+            const float2 v0 = unpack_half(a[2 * c]), v1 = unpack_half(a[2 * c + 1]);
+            const float v[4] = {v0.x, v1.x, v0.y, v1.y};
+            if (!FOLD) mma_tf32(d, v, ako::bf16_lo(bl[2 * u + c]), ako::bf16_hi(bl[2 * u + c]));
+            mma_tf32(d, v, ako::bf16_lo(bh[2 * u + c]), ako::bf16_hi(bh[2 * u + c]));
+          }
+        });
+      }
       if (RINGED) {
         if (tile + 2 * along < te) {
           locate(tile + 2 * along);
@@ -600,8 +638,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, FP8)) paged_decode_ker
     auto finish_ml = [&](int h, float m, float l) {
       if (h >= heads) return;
       const int64_t head = head0 + h;
-      if (whole) p.lse[(int64_t)b * p.q_heads + head] = l == 0.f ? -INFINITY : m + log2f(l);
-      else *reinterpret_cast<float2*>(p.part_ml + (at * p.q_heads + head) * 2) = make_float2(m, l);
+      if (whole) p.lse[(int64_t)b * p.q_heads + head] = l == 0.f ? -INFINITY : (m - LIFT) + log2f(l);
+      else *reinterpret_cast<float2*>(p.part_ml + (at * p.q_heads + head) * 2) = make_float2(m - LIFT, l);
     };
     if (along == 1) {
       const float i0 = l0 == 0.f ? 0.f : 1.f / l0, i1 = l1 == 0.f ? 0.f : 1.f / l1;
