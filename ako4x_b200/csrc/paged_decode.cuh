@@ -14,8 +14,8 @@
 //   * V in registers like K, or, for e4m3 and for 256 features, two tiles of it in shared memory by asynchronous copies that a
 //     lane reads back itself (128 sequences in e4m3: all in registers 235 to 249 us, V in shared memory 218, K too 223;
 //     three of up to 131 072 with 256 features, K and V there: 35, V alone 31).
-//   * P goes in as two pieces, of bf16, which have the exponents of fp32, so that a weight counts however small it is beside
-//     the others; both are positive for a positive weight, so that an infinite value stays infinite: hi = P cut to its leading bits,
+//   * P goes in as two pieces, of bf16, which have the exponents of fp32: both hold what they should down to a weight (times its scale)
+//     of 2^-110. Both are positive for a positive weight, so that an infinite value stays infinite: hi = P cut to its leading bits,
 //     lo = the rest. One piece would put its own rounding beside the output's, and more of it the fewer keys there are.
 //   * Groups of four query heads and fewer leave half of the eight columns free: the second piece of P goes there, and the
 //     accumulators of the two halves are added at the end (64 sequences of up to 8 192 tokens 166 -> 161 us).
@@ -37,11 +37,12 @@
 // several warps take a pair's tiles in turn and put their parts together in shared memory. A share that ends inside a sequence leaves a partial (m, l, O)
 // for the merge kernel.
 //
-// Measured, whole calls: 64 sequences of up to 8 192 tokens, 32 heads over 8 of 128, bf16 (1.03 GB) 160 to 165 us, 6.3 to
-// 6.5 TB/s, 0.96 to 0.99 of the copy rate. 128 of them in e4m3 (1.19 GB) 209 to 220, 0.83 to 0.87: at full clocks 196 to 215, but this
-// one runs into the power limit (1.6 GHz), and fewer instructions are what helps. Three of up to 131 072 tokens, seven heads over
-// one of 256, fp16 (98 MB) 31, half the rate: five tiles to a warp, which the start, the join and the merge (10) outlast.
-// One of 41 tokens 5.3, 5.9 with a warp to a pair, 8.1 with shares and merge.
+// Measured, whole calls, over several GPUs of one kind: 64 sequences of up to 8 192 tokens, 32 heads over 8 of 128, bf16 (1.03 GB) 160 to
+// 167 us, 6.2 to 6.5 TB/s, 0.945 to 0.99 of the copy rate. 128 of them in e4m3 (1.19 GB) 203 to 227, 0.80 to 0.90, 116 M instructions at 0.59 of
+// the issue rate: it runs into the power limit on some (1.6 GHz), and fewer instructions are what helps there. Three of up to 131 072
+// tokens, seven heads over one of 256, fp16 (98 MB) 31, half the rate: five tiles to a warp, which the start, the join and the merge (10)
+// outlast; in e4m3 39 (50 MB). One of 41 tokens 5.3, 5.9 with a warp to a pair, 8.1 with shares and merge. More than eight heads to a KV head
+// take K and V once for every eight of them: 64 x 8 192, 32 heads over 2 of 128 (252 MB) 70, in e4m3 (128 MB) 55.
 #pragma once
 #include <algorithm>
 #include <cfloat>
@@ -187,8 +188,7 @@ __device__ __forceinline__ void empty_head(const Params& p, int64_t row_head) { 
 }
 
 // Where the tiles under way are: K in registers; V too, or (e4m3, whose work on a tile is a long chain, and 256
-// features, which are too many registers) two tiles of it in shared memory. Not K as well: an SM takes a 512-byte
-// asynchronous copy every 20 cycles or so, which is 5.6 TB/s for the GPU.
+// features, which are too many registers) two tiles of it in shared memory. Not K as well, which was slower (above).
 __host__ __device__ constexpr bool ringed(int64_t d, bool fp8) { return fp8 || d == 256; }
 __host__ __device__ constexpr int ctas_per_sm(int64_t d, bool fp8) { return d == 256 && !fp8 ? 2 : 3; }
 // Blocks of a tile: two in e4m3 (64 and 128 features).

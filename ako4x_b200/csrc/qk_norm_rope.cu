@@ -21,9 +21,12 @@
 // 40 rotated: 86 and 54. For all sizes the smaller pieces are not better: 48 us for the next paragraph's 45).
 // Measured, 8 192 tokens with 32 + 8 + 8 heads of 128 into a bf16 cache (201 MB): one piece per lane and partners by
 // shuffle 72 us; two pieces 61; grid without divisions, tables from whole vectors 51; loads ahead across the kinds of
-// rows, 20 warps to an SM 43 to 45 (4.5 to 4.7 TB/s). The same without arithmetic 31: what is left are some 260 instructions
-// for a row group, at half the issue rate. Angles in shared memory for a CTA's tokens instead of tables in registers: 49 to 63; the
-// next row's norm beside this row's rotation: 46; packed fp32 pairs (fma.rn.f32x2): the moves outweigh them.
+// rows, 20 warps to an SM 43 to 45 (4.5 to 4.7 TB/s). The same without arithmetic 31. What is left is neither HBM (0.69 of the copy
+// rate) nor issue slots (257 instructions for a row group, 0.58 of the rate): it is latency, of the loads first, that 20 warps do
+// not cover, and five CTAs to an SM leave 96 registers a thread, of which the forms with pieces of 16 bytes spill 74 bytes (half
+// pairs) or 98 (interleaved). Into an e4m3 cache (185 MB) 52, with 338 instructions a row group, sixteen divisions of a lane and row
+// among them; without norms 44 and 49; rotation alone 36 (168 MB). Angles in shared memory for a CTA's tokens instead of tables in
+// registers: 49 to 63; the next row's norm beside this row's rotation: 46; packed fp32 pairs (fma.rn.f32x2): the moves outweigh them.
 #include <algorithm>
 
 #include "common.cuh"
